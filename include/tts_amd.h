@@ -9,7 +9,8 @@
  *
  * Each declaration cites the reference interface (coqui-ai/TTS v0.22.0, paths relative to the
  * reference root) that it replaces.  Layout everywhere: fp32, channels-first `[B, C, T]`
- * contiguous, exactly like the reference's tensors.
+ * contiguous, exactly like the reference's tensors — except the operators of autoregressive decoding at the end of this file,
+ * which are token-major and take three element types.
  */
 #ifndef TTS_AMD_H
 #define TTS_AMD_H
@@ -664,6 +665,109 @@ int ttsamd_add_row_bias(float *y, const float *x, const float *row_bias, int64_t
  * (align_corners=False, the given scale factor drives the coordinate map) — HifiDecoder.forward,
  * TTS/tts/layers/xtts/hifigan_decoder.py:688-700.  x [rows, t_in] -> y [rows, t_out], t_out = floor(t_in * s). */
 int ttsamd_linear_interp(float *y, const float *x, int64_t rows, int t_in, int t_out, double scale_factor, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Autoregressive decoding: the operators of a decoder layer's step over a paged key/value cache.
+ * serves: the GPT half of XTTS streaming (TTS/tts/models/xtts.py:610-692: one chunk for the prompt, then one audio token at a
+ *   time per request, keys and values of all earlier positions kept), which the reference leaves to a third-party library.
+ * Token-major tensors [tokens, heads, head_dim]: the last dimension contiguous, tokens and heads at any stride (in elements).
+ * All requests of a step travel in one call; sequence b owns the tokens q_starts[b] .. q_starts[b+1]-1.
+ * ---------------------------------------------------------------------------------------- */
+#define TTSAMD_F32 0
+#define TTSAMD_F16 1
+#define TTSAMD_BF16 2
+
+/* Rotary positions: pair i of a head turns by positions * turns[i].  `turns` (device, uint64 [rotary_dim/2]): the pair's turn per
+ * position as a fraction of a full circle in units of 2^-64, so that position * turns wraps exactly where the angle does and far
+ * positions lose nothing.  The first rotary_dim channels of a head turn (pairs (i, i + rotary_dim/2), or (2i, 2i+1) when
+ * interleaved), times `amplitude`; the others are copied. */
+typedef struct ttsamd_rotary_plan {
+    const uint64_t *turns;
+    int32_t rotary_dim;     /* even, <= head_dim */
+    int32_t interleaved;
+    float amplitude;
+} ttsamd_rotary_plan;
+
+typedef struct ttsamd_rotary_args {
+    const void *x;
+    void *y;                              /* may be x itself (same strides) */
+    int64_t x_tstride, x_hstride, y_tstride, y_hstride;
+    const void *positions;                /* [tokens] */
+    int32_t position_bytes;               /* 4 or 8: int32 or int64; any sign */
+    int32_t tokens, heads, head_dim, dtype;
+    int32_t inverse;                      /* turn backwards: the gradient (rotation is orthogonal; amplitude stays a factor) */
+} ttsamd_rotary_args;
+int ttsamd_rotary(const ttsamd_rotary_args *args /* host */, const ttsamd_rotary_plan *plan /* host */, void *stream);
+
+/* A paged cache of one layer: pages [pages][kv_heads][page_size][head_dim] (any strides, in elements; rows contiguous). */
+typedef struct ttsamd_paged_kv {
+    void *k, *v;
+    int64_t k_page, k_head, k_row, v_page, v_head, v_row;
+    int32_t dtype, pages, kv_heads, page_size, head_dim;
+} ttsamd_paged_kv;
+/* The sequences of a call.  seq_lens[b] counts all tokens of sequence b, the new ones included: its new token i sits at position
+ * p = seq_lens[b] - n_b + i, n_b = q_starts[b+1] - q_starts[b], in row p % page_size of page block_table[b][p / page_size].
+ * max_new and max_len (0: what the table can hold) are what the launch is sized by (any n_b and length is still computed whole).  Everything is bounded on the
+ * device: starts are clamped to the tokens of the call, and a position that is negative, behind the table's width or on a page
+ * outside [0, pages) holds no key and takes no write (-1 marks a column without a page). */
+typedef struct ttsamd_paged_batch {
+    const int32_t *block_table;           /* [batch, table_width], row stride table_stride */
+    int64_t table_stride;
+    const int32_t *seq_lens;              /* [batch] */
+    const int32_t *q_starts;              /* [batch + 1] */
+    int32_t table_width, batch, max_new, max_len;
+} ttsamd_paged_batch;
+
+/* Writes the new tokens' keys and values into the cache, the keys (and the queries, if given) rotated on the way, as one launch.
+ * plan NULL: nothing rotates.  positions NULL: a token turns by its place in the cache; else by positions[token].
+ * Element type of every tensor = the cache's.  No two tokens of a call may share a place of the cache. */
+typedef struct ttsamd_kv_append_args {
+    const void *k, *v;                    /* [tokens, kv_heads, head_dim] */
+    int64_t k_tstride, k_hstride, v_tstride, v_hstride;
+    const void *q;                        /* [tokens, q_heads, head_dim], or NULL */
+    void *q_out;                          /* rotated q; may be q itself (same strides) */
+    int64_t q_tstride, q_hstride, qo_tstride, qo_hstride;
+    const void *positions;
+    int32_t position_bytes, tokens, q_heads;
+} ttsamd_kv_append_args;
+int ttsamd_kv_append(const ttsamd_kv_append_args *args /* host */, const ttsamd_paged_kv *cache /* host */,
+                     const ttsamd_paged_batch *batch /* host */, const ttsamd_rotary_plan *plan /* host or NULL */, void *stream);
+
+/* Attention of the new tokens over the cache: out[t,h] = softmax_j(scale * q[t,h] . k_j) v_j over the keys j of t's sequence that
+ * hold a key, with j <= p when causal != 0 and j > p - window when window > 0; p = t's position.  Query head h reads key head
+ * h / (q_heads / kv_heads).  A row that sees no key is zero.  Rows of `out` behind the last sequence are left as they were.
+ * Statistics and sums in fp32.  head_dim a multiple of 8 up to 256; q, out and the cache start and stride at 16 bytes.
+ * `workspace` (device, ttsamd_paged_attention_workspace_bytes; 16-byte aligned; nothing is kept in it between calls): partial
+ * results where a long cache is split over the chip. */
+typedef struct ttsamd_paged_attention_args {
+    const void *q;                        /* [tokens, q_heads, head_dim] */
+    void *out;
+    int64_t q_tstride, q_hstride, o_tstride, o_hstride;
+    int32_t tokens, q_heads, causal, window;
+    float scale;
+} ttsamd_paged_attention_args;
+size_t ttsamd_paged_attention_workspace_bytes(const ttsamd_paged_attention_args *args, const ttsamd_paged_kv *cache,
+                                              const ttsamd_paged_batch *batch);
+int ttsamd_paged_attention(const ttsamd_paged_attention_args *args /* host */, const ttsamd_paged_kv *cache /* host */,
+                           const ttsamd_paged_batch *batch /* host */, void *workspace, size_t workspace_bytes, void *stream);
+
+/* y[m, n] = sum_k x[m, k] * (level[n, k] - zero[n, k / group]) * scale[n, k / group] + bias[n]: a layer with 4-bit weights for the few
+ * rows of a decoding step.  Levels 0..15; without zero points the zero is 8.  fp32 sums of exact products.
+ * `levels`: the image [ceil(n/16)][ceil(k/128)][4 g][16 r][4 j] of 32-bit words; word (g, r, j) of tile (t, c) holds the levels of
+ * output 16 t + r at k = 128 c + 32 j + 8 g + e, e = 0..7, level e in bits 4e .. 4e+3.  `scales` / `zeros`: [ceil(n/16)][groups of the
+ * padded k][16 r], scales in scale_dtype, zeros uint8 (or NULL); padding has scale 0.  All three start at 16 bytes. */
+typedef struct ttsamd_linear_w4_args {
+    const void *x;                        /* [m, k], rows at x_stride */
+    void *y;                              /* [m, n], rows at y_stride */
+    int64_t x_stride, y_stride;
+    const uint32_t *levels;
+    const void *scales;
+    const uint8_t *zeros;
+    const void *bias;                     /* [n] in dtype, or NULL */
+    int32_t m, n, k, group;               /* group 32, 64 or 128; k a multiple of it */
+    int32_t dtype, scale_dtype;
+} ttsamd_linear_w4_args;
+int ttsamd_linear_w4(const ttsamd_linear_w4_args *args /* host */, void *stream);
 
 #ifdef __cplusplus
 }

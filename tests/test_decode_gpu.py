@@ -1,0 +1,376 @@
+"""GPU parity of the autoregressive-decoding operators (rotary positions, the append to a paged cache, attention over it, 4-bit
+products) against oracle/decode.py in 64 bits.
+
+Tolerances.  u = half a step of the type (finfo.eps / 2), f = 2^-24.  A result rounds once: u |y|.  Before that
+  rotary   the angle is off by at most 1.6 f, the Taylor sums by 1.5 f, the factor and the two products by 2 f: 8 f A (|x1| + |x2|)
+  attend   a score is a sum of d products in fp32, off by 6 sqrt(d) f (six sigma of as many roundings) of sum |q k| scale, plus 4 f of it
+           for the scale and the exponential's argument: delta; p is off by delta up and down the softmax: 2 delta, plus 6 sqrt(n) f for
+           its sums over n keys, plus u where p itself is rounded to the 16-bit type: all of it times sum p |v|
+  w4       products are exact but for the level offset of at most 31 in 24 bits: 6 sqrt(k) f of 8 sum |x w|  (an offset level is at most
+           31 against a mean |level - zero| of about 4)"""
+import math
+
+import pytest
+import torch
+
+from oracle import decode as O
+from tts_amd import _lib, ops
+
+pytestmark = pytest.mark.gpu
+F = 2.0 ** -24
+TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _g(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _within(got, want, tol, what=""):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape
+    off = (got - want).abs()
+    bad = ~(off <= tol) & ~(torch.isnan(got) & torch.isnan(want)) & ~(got == want)
+    assert not bool(bad.any()), "%s: %d values off, worst %.3g over its bound (value %.6g, wanted %.6g)" % (
+        what, int(bad.sum()), float((off - tol)[bad].max()), float(got[bad][0]), float(want[bad][0]))
+
+
+# ---------------------------------------------------------------------------------------------------------------- rotary
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("tokens,heads,dim,rd,inter,scaling", [
+    (1, 1, 2, 2, False, None), (3, 5, 64, 64, False, None), (7, 3, 80, 40, True, {"kind": "linear", "factor": 4.0}),
+    (33, 2, 98, 34, False, {"kind": "base", "factor": 8.0}), (5, 16, 128, 0, False, None), (1000, 9, 48, 48, True, None),
+    (2, 4, 256, 128, False, {"kind": "ramp", "factor": 8.0, "trained_len": 4096}), (700, 32, 128, 128, False, None)])
+def test_rotary(gpu, dtype, tokens, heads, dim, rd, inter, scaling):
+    g = _g(tokens + dim)
+    x = torch.randn(tokens, heads, dim, generator=g).to(dtype)
+    pos = torch.randint(-5, 3_000_000, (tokens,), generator=g)
+    plan = ops.Rotary(dim, rd, interleaved=inter, scaling=scaling, device=gpu)
+    rope = [10000.0 ** (-2.0 * i / rd) for i in range(rd // 2)]
+    amp = 1.0
+    if scaling and scaling["kind"] == "linear":
+        rope = [f / 4.0 for f in rope]
+    elif scaling and scaling["kind"] == "base":
+        rope = [(10000.0 * 8.0 ** (rd / (rd - 2.0))) ** (-2.0 * i / rd) for i in range(rd // 2)]
+    elif scaling:
+        keep = [min(1.0, max(0.0, (4096 * f / (2 * math.pi) - 1.0) / 31.0)) for f in rope]
+        rope, amp = [f / 8.0 * (1 - k) + f * k for f, k in zip(rope, keep)], 0.1 * math.log(8.0) + 1.0
+    want = O.turned(x, pos, rope, amp, inter)
+    mag = O.turned(x, torch.zeros_like(pos), rope, amp, inter).abs()
+    pair = mag.clone()
+    if rd:
+        one, two = (slice(0, rd, 2), slice(1, rd, 2)) if inter else (slice(0, rd // 2), slice(rd // 2, rd))
+        pair[..., one] = pair[..., two] = mag[..., one] + mag[..., two]
+    # 2.3e-10: a position of 3e6 times a frequency rounded in 53 bits, in radians
+    tol = u(dtype) * want.abs() * (1 + 8 * F) + pair * (8 * F + 1e-9) + torch.finfo(dtype).tiny
+    got = ops.rotary(plan, x.to(gpu), pos.to(gpu))
+    _within(got, want, tol, "rotary")
+    assert torch.equal(got[..., rd:].cpu(), x[..., rd:])
+    # in place, int32 positions: the same bits
+    y = x.to(gpu).clone()
+    assert ops.rotary(plan, y, pos.to(gpu).int(), out=y) is y and torch.equal(y, got)
+    # strided, unaligned rows in and out: the same bits
+    wide = torch.zeros(tokens, heads + 1, dim + 3, dtype=dtype, device=gpu)
+    wide[:, 1:, 1: dim + 1] = x.to(gpu)
+    out = torch.full((tokens, heads, dim + 5), 7.0, dtype=dtype, device=gpu)
+    ops.rotary(plan, wide[:, 1:, 1: dim + 1], pos.to(gpu), out=out[..., 3: dim + 3])
+    assert torch.equal(out[..., 3: dim + 3], got) and bool((out[..., :3] == 7).all()) and bool((out[..., dim + 3:] == 7).all())
+
+
+def test_rotary_gradient_is_the_inverse_turn(gpu):
+    """<rotary(x), w> has the gradient rotary(w, inverse): against autograd of the plain formula, and against differences."""
+    g = _g(5)
+    x, w = (torch.randn(6, 3, 32, generator=g) for _ in range(2))
+    pos = torch.randint(0, 5000, (6,), generator=g)
+    plan = ops.Rotary(32, 16, interleaved=True, device=gpu)
+    freq = [10000.0 ** (-2.0 * i / 16) for i in range(8)]
+    leaf = x.double().requires_grad_()
+    a = pos.double()[:, None, None] * torch.tensor(freq, dtype=torch.float64)
+    x1, x2 = leaf[..., 0:16:2], leaf[..., 1:16:2]
+    y = torch.cat([torch.stack([x1 * a.cos() - x2 * a.sin(), x2 * a.cos() + x1 * a.sin()], -1).flatten(-2), leaf[..., 16:]], -1)
+    (y * w.double()).sum().backward()
+    got = ops.rotary(plan, w.to(gpu), pos.to(gpu), inverse=True)
+    _within(got, leaf.grad, 8 * F * (w.double().abs().amax() * 2 + leaf.grad.abs()), "gradient")
+    # differences: the map is linear, so a step of any size is exact but for rounding
+    d = torch.randn(6, 3, 32, generator=g)
+    f = lambda t: (ops.rotary(plan, t.to(gpu), pos.to(gpu)).double().cpu() * w.double()).sum()  # noqa: E731
+    slope = float(f(x + d) - f(x - d)) / 2
+    n = x.numel()
+    assert abs(slope - float((got.double().cpu() * d.double()).sum())) <= 64 * F * math.sqrt(n) * float(d.abs().max() + x.abs().max()) * float(w.abs().max())
+
+
+# ------------------------------------------------------------------------------------------------------------ the cache
+class Case:
+    """Sequences with pages dealt out at random from a pool; what no sequence owns holds NaN and infinities."""
+
+    def __init__(self, gpu, dtype, new, lens, kv_heads, heads, dim, page, seed=0, trailing=0, table_extra=0, far_pages=0):
+        g = _g(seed)
+        self.new, self.lens, self.dtype, self.page, self.gpu = list(new), list(lens), dtype, page, gpu
+        owned = [-(-max(c, 0) // page) for c in lens]
+        pages = sum(owned) + 2 + far_pages
+        order = torch.randperm(pages, generator=g)
+        width = max(owned + [0]) + table_extra
+        self.table = torch.full((len(lens), width), -1, dtype=torch.int32)
+        at = 0
+        self.k, self.v = (torch.randn(pages, kv_heads, page, dim, generator=g).to(dtype) for _ in range(2))
+        trash = torch.tensor([math.nan, math.inf, -math.inf])
+        used = torch.zeros(pages, page, dtype=torch.bool)
+        for b, c in enumerate(lens):
+            for i in range(owned[b]):
+                self.table[b, i] = order[at]
+                used[order[at], : min(page, c - i * page)] = True
+                at += 1
+        for c in (self.k, self.v):
+            junk = trash[torch.randint(0, 3, c.shape, generator=g)].to(dtype)
+            c.copy_(torch.where(used[:, None, :, None], c, junk))
+        self.starts = torch.tensor([0] + list(torch.tensor(self.new).cumsum(0)), dtype=torch.int32)
+        self.tokens = sum(self.new) + trailing
+        self.q = torch.randn(self.tokens, heads, dim, generator=g).to(dtype)
+        self.cache = ops.PagedKV(self.k.to(gpu), self.v.to(gpu))
+        self.batch = ops.PagedBatch(self.table.to(gpu), torch.tensor(lens, dtype=torch.int32).to(gpu), self.starts.to(gpu), max(self.new + [0]),
+                                    max(lens + [0]))
+
+    def want(self, scale, causal=True, window=0):
+        return O.attend(self.q, self.cache.k.cpu(), self.cache.v.cpu(), self.table.tolist(), self.lens, self.starts.tolist(), scale, causal, window)
+
+    def check(self, got, scale=None, causal=True, window=0, what=""):
+        dim = self.q.shape[2]
+        scale = dim ** -0.5 if scale is None else scale
+        want, mag, reach = self.want(scale, causal, window)
+        delta = (6 * math.sqrt(dim) + 4) * F * reach
+        rel = 2 * delta + 6 * math.sqrt(max(self.lens + [1])) * F + (u(self.dtype) if self.dtype != torch.float32 else 0.0) + 8 * F
+        mine = ~torch.isnan(want).all(-1).all(-1)
+        _within(got[mine.to(got.device)], want[mine], u(self.dtype) * want[mine].abs() + rel * mag[mine] + torch.finfo(self.dtype).tiny, what)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("new,lens,kv,heads,dim,page,rd,inter", [
+    ([1], [1], 1, 1, 8, 1, 8, False), ([1, 1, 1], [17, 16, 1], 2, 4, 64, 16, 64, False), ([5, 0, 3], [5, 9, 40], 1, 3, 40, 7, 20, True),
+    ([130, 1, 77], [130, 300, 90], 4, 4, 128, 32, 64, False), ([300], [300], 8, 16, 256, 64, 0, False)])
+def test_kv_append(gpu, dtype, new, lens, kv, heads, dim, page, rd, inter):
+    c = Case(gpu, dtype, new, lens, kv, heads, dim, page, seed=dim + page, trailing=2)
+    g = _g(9)
+    k, v = (torch.randn(c.tokens, kv, dim, generator=g).to(dtype) for _ in range(2))
+    plan = ops.Rotary(dim, rd, interleaved=inter, device=gpu)
+    before_k, before_v = c.cache.k.cpu().clone(), c.cache.v.cpu().clone()
+    q = ops.kv_append(c.cache, c.batch, k.to(gpu), v.to(gpu), rotary=plan, q=c.q.to(gpu))
+    got_k, got_v = c.cache.k.cpu(), c.cache.v.cpu()
+    own = sum(new)
+    pos = torch.cat([torch.arange(n - a, n) for a, n in zip(new, lens)])
+    # the rotation is rotary()'s own, bit for bit (itself held to 64 bits above)
+    want_k = ops.rotary(plan, k[:own].to(gpu), pos.to(gpu)).cpu()
+    assert torch.equal(q[:own].cpu(), ops.rotary(plan, c.q[:own].to(gpu), pos.to(gpu)).cpu())
+    at = 0
+    for b, (start, n, where, slots) in enumerate(O.places(c.table.tolist(), lens, c.starts.tolist(), page, c.k.shape[0], c.tokens)):
+        for i in range(n):
+            pg, row = slots[where[i]]
+            before_k[pg, :, row], before_v[pg, :, row] = want_k[start + i], v[start + i]
+            at += 1
+    assert at == own
+    same = lambda a, b: torch.equal(a.view(torch.int16 if dtype != torch.float32 else torch.int32), b.view(torch.int16 if dtype != torch.float32 else torch.int32))  # noqa: E731,E501
+    assert same(got_k, before_k) and same(got_v, before_v)          # every other row of the cache as it was, NaN and all
+    # without a plan nothing turns; positions of the caller's own
+    ops.kv_append(c.cache, c.batch, k.to(gpu), v.to(gpu))
+    where = [s[p] for _, n, w, s in O.places(c.table.tolist(), lens, c.starts.tolist(), page, c.k.shape[0], c.tokens) for p in w]
+    assert all(torch.equal(c.cache.k.cpu()[pg, :, r], k[i]) for i, (pg, r) in enumerate(where))
+    other = torch.arange(c.tokens) * 3 - 4
+    ops.kv_append(c.cache, c.batch, k.to(gpu), v.to(gpu), rotary=plan, positions=other.to(gpu))
+    turned = ops.rotary(plan, k.to(gpu), other.to(gpu)).cpu()
+    assert all(torch.equal(c.cache.k.cpu()[pg, :, r], turned[i]) for i, (pg, r) in enumerate(where))
+
+
+def test_kv_append_takes_no_write_outside_the_pages(gpu):
+    """Pages that are not there, positions before the first and behind the table: those tokens write nothing; the others all do."""
+    new, lens = [4, 3, 2], [2, 12, 9]                                # sequence 0: two tokens at positions -2, -1
+    c = Case(gpu, torch.float32, new, lens, 2, 2, 16, 4, seed=3)
+    c.table[1, 2] = c.k.shape[0] + 5                                 # positions 8..11 of sequence 1: no such page
+    table = c.table[:, :2].contiguous().to(gpu)                      # sequence 2's position 8 is behind the table
+    c.table[1, 2] = -7
+    for t, page1 in ((table, -1), (c.table.to(gpu), -7)):
+        cache = ops.PagedKV.allocate(c.k.shape[0], 4, 2, 16, device=gpu)
+        batch = ops.PagedBatch(t, c.batch.seq_lens, c.batch.q_starts, 4)
+        k = torch.randn(9, 2, 16, generator=_g(1)).to(gpu)
+        ops.kv_append(cache, batch, k, -k)
+        want = torch.zeros_like(cache.k)
+        for start, n, pos, where in O.places(t.tolist(), lens, c.starts.tolist(), 4, c.k.shape[0], 9):
+            for i, p in enumerate(pos):
+                if p >= 0 and where[p] is not None:
+                    want[where[p][0], :, where[p][1]] = k[start + i]
+        assert torch.equal(cache.k, want) and torch.equal(cache.v, -want)
+
+
+# --------------------------------------------------------------------------------------------------------- attention
+ATTEND = [
+    # new, lens, kv_heads, heads, dim, page: single tokens
+    ([1], [1], 1, 1, 8, 1), ([1], [2], 1, 1, 64, 16), ([1, 1, 1, 1], [63, 64, 65, 1], 2, 2, 64, 16), ([1, 1], [0, 5], 2, 4, 64, 4),
+    ([1, 1], [1000, 777], 2, 6, 128, 64), ([1], [5000], 1, 8, 64, 32), ([1, 1, 0, 1], [129, 31, 40, 256], 1, 16, 80, 24),
+    ([1], [700], 2, 34, 96, 16), ([1, 1], [300, 50], 1, 1, 256, 128), ([1], [513], 3, 3, 40, 7),
+    # chunks
+    ([2], [2], 1, 1, 64, 16), ([17, 1, 33], [17, 40, 33], 2, 2, 64, 16), ([5, 64], [100, 64], 1, 3, 128, 1), ([70], [333], 2, 4, 72, 24),
+    ([129, 128, 127], [129, 200, 500], 1, 2, 128, 64), ([40], [40], 1, 8, 256, 16), ([300], [310], 2, 2, 32, 13), ([9, 6], [4, 6], 1, 2, 64, 8)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("new,lens,kv,heads,dim,page", ATTEND)
+def test_paged_attention(gpu, dtype, new, lens, kv, heads, dim, page):
+    c = Case(gpu, dtype, new, lens, kv, heads, dim, page, seed=sum(lens) + dim, trailing=3, table_extra=1)
+    out = torch.full(c.q.shape, 5.0, dtype=dtype, device=gpu)
+    got = ops.paged_attention(c.q.to(gpu), c.cache, c.batch, out=out)
+    assert got is out and bool((out[sum(new):] == 5).all())           # behind the last sequence: as it was
+    c.check(got, what="causal")
+    got = ops.paged_attention(c.q.to(gpu), c.cache, c.batch, window=max(1, max(lens) // 3), scale=0.3)
+    c.check(got, scale=0.3, window=max(1, max(lens) // 3), what="window")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("new,lens,window", [([1, 1], [200, 33], 0), ([40, 3], [200, 33], 0), ([40, 90], [200, 90], 50), ([1], [90], 1)])
+def test_paged_attention_not_causal(gpu, dtype, new, lens, window):
+    c = Case(gpu, dtype, new, lens, 2, 4, 64, 16, seed=7)
+    c.check(ops.paged_attention(c.q.to(gpu), c.cache, c.batch, causal=False, window=window), causal=False, window=window)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("new", [1, 20, 150])
+def test_paged_attention_bad_pages_and_sizes_hold_no_key(gpu, dtype, new):
+    """Pages outside the pool, a table narrower than the lengths, starts beyond the tokens: what is there is attended, nothing faults."""
+    c = Case(gpu, dtype, [new, new], [160, 170], 2, 4, 64, 16, seed=new)
+    for col, page in ((0, -3), (3, 10 ** 6), (9, 2 ** 31 - 1)):
+        c.table[0, col] = page
+    c.table = c.table[:, :10].contiguous()                            # sequence 1 reaches position 169: its last keys have no column
+    c.batch = ops.PagedBatch(c.table.to(gpu), c.batch.seq_lens, c.batch.q_starts, new)
+    c.check(ops.paged_attention(c.q.to(gpu), c.cache, c.batch), what="pages")
+    c.table[1, :] = -1                                                # a sequence with no page at all: zeros
+    c.batch = ops.PagedBatch(c.table.to(gpu), c.batch.seq_lens, c.batch.q_starts, new)
+    got = ops.paged_attention(c.q.to(gpu), c.cache, c.batch)
+    assert bool((got[new:] == 0).all())
+    c.check(got, what="no page")
+    c.starts = torch.tensor([-4, new + 3, 10 ** 9], dtype=torch.int32)
+    c.batch = ops.PagedBatch(c.table.to(gpu), c.batch.seq_lens, c.starts.to(gpu), new)
+    c.check(ops.paged_attention(c.q.to(gpu), c.cache, c.batch), what="starts")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_paged_attention_computes_more_than_it_was_sized_for(gpu, dtype):
+    c = Case(gpu, dtype, [70, 1, 200], [90, 400, 250], 2, 4, 64, 16, seed=2)
+    for most in ((1, 1), (0, 0), (7, 40)):
+        c.batch = ops.PagedBatch(c.table.to(gpu), c.batch.seq_lens, c.batch.q_starts, max_new=most[0], max_len=most[1])
+        c.check(ops.paged_attention(c.q.to(gpu), c.cache, c.batch), what=str(most))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("new", [1, 90])
+def test_paged_attention_strides_and_large_scores(gpu, dtype, new):
+    """A layer's slice of a cache of many layers, q as a slice of one projection, out in a wider tensor; scores in the hundreds."""
+    c = Case(gpu, dtype, [new, new], [300, 120], 2, 4, 64, 16, seed=4)
+    pages = c.k.shape[0]
+    pool = torch.full((pages, 3, 2, 16, 2, 64), math.nan, dtype=dtype, device=gpu)    # [pages, layers, k/v, rows, heads, dim]
+    pool[:, 1, 0], pool[:, 1, 1] = c.k.to(gpu).transpose(1, 2), c.v.to(gpu).transpose(1, 2)
+    cache = ops.PagedKV(pool[:, 1, 0].transpose(1, 2), pool[:, 1, 1].transpose(1, 2))
+    fused = torch.randn(c.tokens, 8, 64, generator=_g(1)).to(dtype).to(gpu)
+    fused[:, 2:6] = (c.q * 20).to(gpu)
+    wide = torch.full((c.tokens, 6, 64), 3.0, dtype=dtype, device=gpu)
+    ops.paged_attention(fused[:, 2:6], cache, c.batch, out=wide[:, 1:5])
+    assert bool((wide[:, 0] == 3).all()) and bool((wide[:, 5] == 3).all())
+    c.q = fused[:, 2:6].cpu()
+    c.check(wide[:, 1:5], what="strided")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_paged_attention_non_finite_values_reach_only_who_sees_them(gpu, dtype):
+    """NaN and infinities in keys or values of tokens that a row does not see (later ones of its chunk, those out of its window) take no
+    part in it."""
+    new, n = 100, 180
+    c = Case(gpu, dtype, [new], [n], 1, 2, 64, 16, seed=8)
+    for j, value in ((120, math.nan), (150, math.inf), (171, -math.inf)):
+        page, row = int(c.table[0, j // 16]), j % 16
+        (c.cache.k if j == 150 else c.cache.v)[page, :, row, 5] = value
+    for window in (0, 20):
+        got = ops.paged_attention(c.q.to(gpu), c.cache, c.batch, window=window)
+        want, _, _ = c.want(64 ** -0.5, True, window)
+        assert torch.equal(torch.isfinite(got).cpu(), torch.isfinite(want)), window
+        fine = [i for i in range(new) if bool(torch.isfinite(want[i]).all())]
+        assert len(fine) >= 40
+        sub = got[fine].double().cpu() - want[fine]
+        assert float(sub.abs().max()) < 40 * u(dtype) + 1e-5
+
+
+def test_paged_attention_positions_beyond_32_bits_of_bytes(gpu):
+    """A pool whose pages lie further apart than 2^31 elements."""
+    dtype = torch.bfloat16
+    c = Case(gpu, dtype, [1, 30], [100, 70], 1, 2, 64, 16, seed=6)
+    pages = c.k.shape[0]
+    stride = (1 << 31) // (pages - 3) // 8 * 8 + 8
+    pool = torch.empty((pages - 1) * stride + 2 * 16 * 64, dtype=dtype, device=gpu)
+    k = pool.as_strided((pages, 1, 16, 64), (stride, 1024, 64, 1))
+    v = pool[1024:].as_strided((pages, 1, 16, 64), (stride, 1024, 64, 1))
+    k.copy_(c.k.to(gpu)), v.copy_(c.v.to(gpu))
+    assert (pages - 1) * stride * 2 > 1 << 32
+    cache = ops.PagedKV(k, v)
+    c.check(ops.paged_attention(c.q.to(gpu), cache, c.batch))
+    new_k = torch.randn(31, 1, 64, generator=_g(3)).to(dtype).to(gpu)
+    ops.kv_append(cache, c.batch, new_k, new_k)
+    c.cache = ops.PagedKV(k.contiguous(), v.contiguous())
+    c.check(ops.paged_attention(c.q.to(gpu), cache, c.batch))
+    assert torch.equal(cache.k[int(c.table[0, 6]), :, 3], new_k[0])
+
+
+# ------------------------------------------------------------------------------------------------------------------- w4
+def _w4(dtype, m, n, k, group, zeros, bias, seed):
+    g = _g(seed)
+    x = torch.randn(m, k, generator=g).to(dtype)
+    q = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8)
+    s = ((torch.rand(n, k // group, generator=g) + 0.5) / math.sqrt(k)).to(dtype)
+    z = torch.randint(0, 16, (n, k // group), generator=g, dtype=torch.uint8) if zeros else None
+    b = torch.randn(n, generator=g).to(dtype) if bias else None
+    return x, q, s, z, b
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,n,k,group,zeros,bias", [
+    (1, 1, 32, 32, False, False), (1, 16, 128, 128, True, True), (2, 100, 256, 64, False, True), (5, 17, 96, 32, True, False),
+    (1, 1024, 1024, 64, False, True), (16, 33, 640, 128, True, True), (17, 64, 320, 64, False, False), (33, 250, 1056, 32, True, True),
+    (64, 48, 512, 128, False, True), (100, 20, 192, 64, True, False), (1, 40, 8192, 128, False, True), (4, 4096, 64, 64, True, True),
+    (260, 70, 384, 128, False, False)])
+def test_linear_w4(gpu, dtype, m, n, k, group, zeros, bias):
+    x, q, s, z, b = _w4(dtype, m, n, k, group, zeros, bias, m + n + k)
+    want, mag = O.linear_w4(x, q, s, z, b)
+    up = lambda t: None if t is None else t.to(gpu)  # noqa: E731
+    pw = ops.PackedW4(up(q), up(s), up(z), up(b))
+    tol = u(dtype) * want.abs() + 8 * 6 * math.sqrt(k) * F * mag + 2 * F * want.abs() + torch.finfo(dtype).tiny
+    if b is not None:
+        tol = tol + 2 * F * b.double().abs()
+    got = ops.linear_w4(pw, x.to(gpu))
+    _within(got, want, tol, "w4")
+    # rows of a wider x into rows of a wider y
+    wide = torch.full((m, k + 8), 9.0, dtype=dtype, device=gpu)
+    wide[:, 3: k + 3] = x.to(gpu)
+    out = torch.full((m, n + 5), 4.0, dtype=dtype, device=gpu)
+    ops.linear_w4(pw, wide[:, 3: k + 3], out=out[:, 2: n + 2])
+    assert torch.equal(out[:, 2: n + 2], got) and bool((out[:, :2] == 4).all()) and bool((out[:, n + 2:] == 4).all())
+
+
+@pytest.mark.parametrize("scale_dtype", TYPES, ids=str)
+def test_linear_w4_scales_of_any_type_and_non_finite_rows(gpu, scale_dtype):
+    x, q, s, z, _ = _w4(torch.float32, 3, 30, 256, 64, True, False, 1)
+    x[1, 70] = math.nan
+    x[2, 255] = math.inf
+    pw = ops.PackedW4(q.to(gpu), s.to(scale_dtype).to(gpu), z.to(gpu))
+    want, mag = O.linear_w4(x[:1], q, s.to(scale_dtype), z)
+    got = ops.linear_w4(pw, x.to(gpu))
+    _within(got[:1], want, 8 * 6 * 16 * F * mag, "scales")            # a row is its own: NaN and infinity next to it change nothing
+    assert bool(torch.isnan(got[1]).all()) and not bool(torch.isfinite(got[2]).any())
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_quantize_is_within_half_a_step(gpu, group, zeros):
+    w = torch.randn(40, 256, generator=_g(2)).to(gpu)
+    pw = ops.PackedW4.quantize(w, group, zeros=zeros)
+    back = ops.linear_w4(pw, torch.eye(256, device=gpu)).t()
+    f = w.view(40, -1, group)
+    step = (f.amax(-1).clamp(min=0) - f.amin(-1).clamp(max=0)) / 15 if zeros else f.abs().amax(-1) / 7.5
+    # half a step inside the range; with a zero point rounded to a level another half at the ends
+    assert bool(((back - w).abs().view(40, -1, group) <= (1.01 if zeros else 0.51) * step[..., None] + 1e-6).all())

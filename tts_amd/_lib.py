@@ -44,6 +44,7 @@ def lib():
         _lib.ttsamd_last_error.restype = ctypes.c_char_p
         _lib.ttsamd_arch.restype = ctypes.c_char_p
         _lib.ttsamd_maximum_path_workspace_bytes.restype = ctypes.c_size_t
+        _lib.ttsamd_paged_attention_workspace_bytes.restype = ctypes.c_size_t
     return _lib
 
 

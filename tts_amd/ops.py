@@ -773,3 +773,371 @@ def sample_gaussian(stats, noise, mask):
     check(lib().ttsamd_sample_gaussian(P(z), P(stats), P(noise.contiguous()), P(mask), B, C2 // 2, T, stream_ptr()),
           "sample_gaussian")
     return z
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# Autoregressive decoding (include/tts_amd.h, last section): rotary positions, a paged key/value cache, attention over it and
+# products with 4-bit weights.  Token-major [tokens, heads, head_dim] tensors in float32, float16 or bfloat16.  Work is queued on
+# the tensors' device, on its current stream.  All of it can be captured into a graph: nothing waits for the device, and sizes
+# that vary from step to step (lengths, starts, the block table) are read there.
+# ---------------------------------------------------------------------------------------------------------------------
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # TTSAMD_F32 / F16 / BF16
+
+
+class _RotaryPlan(ctypes.Structure):
+    """Mirror of `ttsamd_rotary_plan`."""
+
+    _fields_ = [("turns", ctypes.c_void_p), ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("amplitude", ctypes.c_float)]
+
+
+class _RotaryArgs(ctypes.Structure):
+    """Mirror of `ttsamd_rotary_args`."""
+
+    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("x_tstride", ctypes.c_int64), ("x_hstride", ctypes.c_int64),
+                ("y_tstride", ctypes.c_int64), ("y_hstride", ctypes.c_int64), ("positions", ctypes.c_void_p),
+                ("position_bytes", ctypes.c_int32), ("tokens", ctypes.c_int32), ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("inverse", ctypes.c_int32)]
+
+
+class _PagedKV(ctypes.Structure):
+    """Mirror of `ttsamd_paged_kv`."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
+        [(n, ctypes.c_int64) for n in ("k_page", "k_head", "k_row", "v_page", "v_head", "v_row")] + \
+        [(n, ctypes.c_int32) for n in ("dtype", "pages", "kv_heads", "page_size", "head_dim")]
+
+
+class _PagedBatch(ctypes.Structure):
+    """Mirror of `ttsamd_paged_batch`."""
+
+    _fields_ = [("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("seq_lens", ctypes.c_void_p),
+                ("q_starts", ctypes.c_void_p)] + [(n, ctypes.c_int32) for n in ("table_width", "batch", "max_new", "max_len")]
+
+
+class _KvAppendArgs(ctypes.Structure):
+    """Mirror of `ttsamd_kv_append_args`."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
+        [(n, ctypes.c_int64) for n in ("k_tstride", "k_hstride", "v_tstride", "v_hstride")] + \
+        [("q", ctypes.c_void_p), ("q_out", ctypes.c_void_p)] + \
+        [(n, ctypes.c_int64) for n in ("q_tstride", "q_hstride", "qo_tstride", "qo_hstride")] + \
+        [("positions", ctypes.c_void_p)] + [(n, ctypes.c_int32) for n in ("position_bytes", "tokens", "q_heads")]
+
+
+class _PagedAttentionArgs(ctypes.Structure):
+    """Mirror of `ttsamd_paged_attention_args`."""
+
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p)] + \
+        [(n, ctypes.c_int64) for n in ("q_tstride", "q_hstride", "o_tstride", "o_hstride")] + \
+        [(n, ctypes.c_int32) for n in ("tokens", "q_heads", "causal", "window")] + [("scale", ctypes.c_float)]
+
+
+class _LinearW4Args(ctypes.Structure):
+    """Mirror of `ttsamd_linear_w4_args`."""
+
+    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("y_stride", ctypes.c_int64)] + \
+        [(n, ctypes.c_void_p) for n in ("levels", "scales", "zeros", "bias")] + \
+        [(n, ctypes.c_int32) for n in ("m", "n", "k", "group", "dtype", "scale_dtype")]
+
+
+def _need(ok, message):
+    if not ok:
+        raise _lib.TtsAmdError(message)
+
+
+_FNS = {}
+
+
+def _queue(what, device, *args):
+    """One call of the library's function `what` on the current stream of `device` (made current for the call if it is not)."""
+    fn = _FNS.get(what)
+    if fn is None:
+        fn = _FNS[what] = getattr(lib(), "ttsamd_" + what)
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _queue(what, device, *args)
+    rc = fn(*args, ctypes.c_void_p(torch.cuda.current_stream(index).cuda_stream))
+    if rc:
+        check(rc, what)
+
+
+def _rows(t, what, heads_dim, dtype, device):
+    """A [tokens, heads, head_dim] tensor of the call: checked, its (token, head) strides returned."""
+    _need(t.dim() == 3 and t.shape[1:] == heads_dim, "%s is %s: [tokens, %d, %d] is wanted" % (what, tuple(t.shape), *heads_dim))
+    _need(t.dtype == dtype and t.device == device, "%s is %s on %s: %s on %s is wanted" % (what, t.dtype, t.device, dtype, device))
+    st, sh, sd = t.stride()
+    _need(sd == 1 or t.shape[2] <= 1, "%s: the channels of a head have to be contiguous" % what)
+    return st, sh
+
+
+def _inner(s, shape):
+    """Strides with 0 where a dimension has one entry (whatever torch holds there is never used)."""
+    return [0 if n <= 1 else int(v) for v, n in zip(s, shape)]
+
+
+class Rotary:
+    """The plan of a rotary position encoding: how far each pair of channels turns per position (`ttsamd_rotary_plan`).
+
+    head_dim       channels of a head; the first `rotary_dim` of them turn (default: all), the others pass through
+    base           pair i turns by base ** (-2 i / rotary_dim) radians a position
+    interleaved    pairs are (2i, 2i+1); else (i, i + rotary_dim / 2)
+    scaling        for contexts longer than the model was trained on, a dict with `kind` and `factor`:
+                     linear  every frequency divided by the factor
+                     base    the base times factor ** (rotary_dim / (rotary_dim - 2)): the fastest pair keeps its pace, the slowest
+                             slows by the factor
+                     ramp    pairs that turn more than `high` times within `trained_len` positions keep their pace, those that turn
+                             less than `low` times slow by the factor, blended between; values times `amplitude`
+                             (default 0.1 ln(factor) + 1)
+    inv_freq       the frequencies themselves (radians a position, rotary_dim / 2 of them), instead of base and scaling"""
+
+    def __init__(self, head_dim, rotary_dim=None, base=10000.0, interleaved=False, scaling=None, inv_freq=None, amplitude=None, device="cuda"):
+        import math
+        from fractions import Fraction
+
+        rd = head_dim if rotary_dim is None else rotary_dim
+        _need(rd % 2 == 0 and 0 <= rd <= head_dim, "rotary_dim %d of a head of %d: an even number up to it" % (rd, head_dim))
+        gain = 1.0
+        if inv_freq is not None:
+            _need(scaling is None, "inv_freq already holds the scaling")
+            freq = [float(f) for f in inv_freq]
+            _need(len(freq) == rd // 2, "%d frequencies for %d pairs" % (len(freq), rd // 2))
+        else:
+            sc = dict(scaling or {"kind": "none", "factor": 1.0})
+            kind, factor = sc.pop("kind", None), float(sc.pop("factor", 1.0))
+            _need(kind in ("none", "linear", "base", "ramp"), "scaling kind %r: linear, base or ramp" % (kind,))
+            _need(factor > 0 and base > 0, "base and factor have to be positive")
+            if kind == "base":
+                _need(rd > 2, "scaling the base needs more than one pair")
+                base = base * factor ** (rd / (rd - 2.0))
+            freq = [base ** (-2.0 * i / rd) for i in range(rd // 2)]
+            if kind == "linear":
+                freq = [f / factor for f in freq]
+            elif kind == "ramp":
+                trained, low, high = float(sc.pop("trained_len")), float(sc.pop("low", 1.0)), float(sc.pop("high", 32.0))
+                _need(high > low, "ramp: high has to be above low")
+                keep = [min(1.0, max(0.0, (trained * f / (2 * math.pi) - low) / (high - low))) for f in freq]
+                freq = [f / factor * (1 - r) + f * r for f, r in zip(freq, keep)]
+                gain = float(sc.pop("amplitude", 0.1 * math.log(factor) + 1.0))
+            _need(not sc, "scaling %s does not take %s" % (kind, sorted(sc)))
+        _need(all(math.isfinite(f) for f in freq), "a frequency is not finite")
+        self.head_dim, self.rotary_dim, self.interleaved = head_dim, rd, bool(interleaved)
+        self.amplitude = gain if amplitude is None else float(amplitude)
+        circle = 2 * Fraction(31415926535897932384626433832795028841971693993751, 10 ** 49)
+        turns = [round(Fraction(f) / circle * 2 ** 64) % 2 ** 64 for f in freq]
+        self.turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64).to(device)
+        self.device = self.turns.device
+        self._c = _RotaryPlan(self.turns.data_ptr() if rd else None, rd, int(self.interleaved), self.amplitude)
+        self._ref = ctypes.addressof(self._c)
+
+
+def _positions(positions, tokens, device):
+    _need(positions.dtype in (torch.int64, torch.int32) and positions.is_contiguous() and positions.numel() == tokens,
+          "positions: %d contiguous int64 or int32 values are wanted" % tokens)
+    _need(positions.device == device, "positions are on %s, the tensors on %s" % (positions.device, device))
+    return positions.data_ptr(), positions.element_size()
+
+
+def rotary(plan, x, positions, out=None, inverse=False):
+    """x [tokens, heads, head_dim] with every head turned to its token's position [tokens] (any sign), into `out` (may be x; default: a
+    new tensor).  inverse=True turns back: the gradient of rotary() with respect to x, given the gradient of its result."""
+    _need(x.dim() == 3 and x.dtype in _DTYPES, "x is %s %s: [tokens, heads, head_dim] in float32, float16 or bfloat16 is wanted"
+          % (x.dtype, tuple(x.shape)))
+    tokens, heads, dim = x.shape
+    _need(dim == plan.head_dim, "x has heads of %d channels, the plan of %d" % (dim, plan.head_dim))
+    xt, xh = _rows(x, "x", (heads, dim), x.dtype, x.device)
+    pp, pb = _positions(positions, tokens, x.device)
+    _need(plan.device == x.device, "the plan is on %s, x on %s" % (plan.device, x.device))
+    _lib.require_gpu(x, "x")
+    y = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device) if out is None else out
+    yt, yh = _rows(y, "out", (heads, dim), x.dtype, x.device)
+    _need(y.shape[0] == tokens, "out has %d tokens, x %d" % (y.shape[0], tokens))
+    a = _RotaryArgs(x.data_ptr(), y.data_ptr(), xt, xh, yt, yh, pp, pb, tokens, heads, dim, _DTYPES[x.dtype], int(inverse))
+    _queue("rotary", x.device, ctypes.byref(a), ctypes.c_void_p(plan._ref))
+    return y
+
+
+class PagedKV:
+    """One layer's keys and values in pages: k, v [pages, kv_heads, page_size, head_dim], the caller's own tensors (any strides that are
+    multiples of 16 bytes, channels contiguous).  head_dim: a multiple of 8 up to 256."""
+
+    def __init__(self, k, v):
+        _need(k.dim() == 4 and k.shape == v.shape, "k is %s, v %s: both [pages, kv_heads, page_size, head_dim]" % (tuple(k.shape), tuple(v.shape)))
+        _need(k.dtype in _DTYPES and v.dtype == k.dtype and v.device == k.device, "k and v: one of float32, float16, bfloat16, on one device")
+        pages, heads, rows, dim = k.shape
+        _need(min(k.shape) > 0, "the cache is empty: %s" % (tuple(k.shape),))
+        _need(dim % 8 == 0 and dim <= 256, "heads of %d channels: a multiple of 8 up to 256 is wanted" % dim)
+        _need(k.stride(3) == 1 and v.stride(3) == 1, "the channels of a row have to be contiguous")
+        per = 16 // k.element_size()
+        ks, vs = _inner(k.stride()[:3], k.shape), _inner(v.stride()[:3], v.shape)
+        _need(all(s % per == 0 for s in ks + vs) and k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0,
+              "rows of the cache have to start at multiples of 16 bytes")
+        self.k, self.v, self.dtype, self.device = k, v, k.dtype, k.device
+        self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, rows, dim
+        self._c = _PagedKV(k.data_ptr(), v.data_ptr(), *ks, *vs, _DTYPES[k.dtype], pages, heads, rows, dim)
+        self._ref = ctypes.addressof(self._c)
+
+    @classmethod
+    def allocate(cls, pages, page_size, kv_heads, head_dim, dtype=torch.float32, device="cuda"):
+        return cls(*(torch.zeros((pages, kv_heads, page_size, head_dim), dtype=dtype, device=device) for _ in range(2)))
+
+
+class PagedBatch:
+    """The sequences of a step (`ttsamd_paged_batch`): block_table int32 [batch, width] (a row's pages in order; -1: none), seq_lens int32
+    [batch] (tokens in all, the new ones included), q_starts int32 [batch + 1] (where each sequence's new tokens begin).  All three are
+    read on the device when the work runs, so a captured graph follows what is written into them.  max_new / max_len: the most new
+    tokens / tokens of a sequence, which launches are sized by (max_len default: what the table can hold); longer ones are still computed
+    whole, only on fewer workgroups."""
+
+    def __init__(self, block_table, seq_lens, q_starts, max_new, max_len=None):
+        batch = seq_lens.shape[0]
+        _need(all(t.dtype == torch.int32 for t in (block_table, seq_lens, q_starts)), "block_table, seq_lens and q_starts are int32")
+        _need(block_table.dim() == 2 and block_table.shape[0] == batch and seq_lens.dim() == 1 and tuple(q_starts.shape) == (batch + 1,),
+              "block_table [batch, width], seq_lens [batch], q_starts [batch + 1] are wanted")
+        _need(seq_lens.is_contiguous() and q_starts.is_contiguous() and (block_table.shape[1] <= 1 or block_table.stride(1) == 1),
+              "seq_lens, q_starts and the rows of block_table have to be contiguous")
+        _need(seq_lens.device == block_table.device == q_starts.device, "block_table, seq_lens and q_starts are on one device")
+        _need(batch <= 65535, "%d sequences: up to 65535" % batch)
+        _need(0 <= int(max_new) < 2 ** 31 and (max_len is None or 0 <= int(max_len) < 2 ** 31), "max_new and max_len: 0 .. 2^31 - 1")
+        self.block_table, self.seq_lens, self.q_starts = block_table, seq_lens, q_starts
+        self.batch, self.max_new, self.device = batch, int(max_new), seq_lens.device
+        self._c = _PagedBatch(block_table.data_ptr(), block_table.stride(0) if batch > 1 else 0, seq_lens.data_ptr(), q_starts.data_ptr(),
+                              block_table.shape[1], batch, self.max_new, 0 if max_len is None else int(max_len))
+        self._ref = ctypes.addressof(self._c)
+
+    def _for(self, cache):
+        _need(self.device == cache.device, "the batch is on %s, the cache on %s" % (self.device, cache.device))
+        return ctypes.c_void_p(self._ref)
+
+
+def kv_append(cache, batch, k, v, rotary=None, q=None, positions=None, q_out=None):
+    """Writes k, v [tokens, kv_heads, head_dim] of the batch's new tokens to their places in the cache; with a `rotary` plan the keys, and
+    q [tokens, q_heads, head_dim] if given, turn on the way.  Returns the turned q (in `q_out`, which may be q; default: a new tensor), or
+    None.  Tokens turn by their place in the cache, or by `positions` [tokens].  One launch."""
+    tokens = k.shape[0]
+    kt, kh = _rows(k, "k", (cache.kv_heads, cache.head_dim), cache.dtype, cache.device)
+    vt, vh = _rows(v, "v", (cache.kv_heads, cache.head_dim), cache.dtype, cache.device)
+    _need(v.shape[0] == tokens, "k has %d tokens, v %d" % (tokens, v.shape[0]))
+    a = _KvAppendArgs(k.data_ptr(), v.data_ptr(), kt, kh, vt, vh)
+    a.tokens = tokens
+    if q is not None:
+        _need(q.dim() == 3 and q.shape[0] == tokens and q.shape[1] > 0, "q is %s: [%d, q_heads, head_dim] is wanted" % (tuple(q.shape), tokens))
+        shape = (q.shape[1], cache.head_dim)
+        a.q_tstride, a.q_hstride = _rows(q, "q", shape, cache.dtype, cache.device)
+    else:
+        _need(q_out is None, "q_out without q")
+    if positions is not None:
+        _need(rotary is not None, "positions without a rotary plan")
+        a.positions, a.position_bytes = _positions(positions, tokens, cache.device)
+    if rotary is not None:
+        _need(rotary.head_dim == cache.head_dim and rotary.device == cache.device,
+              "the plan is for heads of %d on %s, the cache has %d on %s" % (rotary.head_dim, rotary.device, cache.head_dim, cache.device))
+    ref = batch._for(cache)
+    _lib.require_gpu(k, "k")
+    if q is not None:
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        else:
+            _need(q_out.shape == q.shape, "q_out is %s, q %s" % (tuple(q_out.shape), tuple(q.shape)))
+        a.qo_tstride, a.qo_hstride = _rows(q_out, "q_out", shape, cache.dtype, cache.device)
+        a.q, a.q_out, a.q_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+    _queue("kv_append", cache.device, ctypes.byref(a), ctypes.c_void_p(cache._ref), ref, ctypes.c_void_p(rotary._ref) if rotary is not None else None)
+    return q_out
+
+
+def paged_attention(q, cache, batch, scale=None, causal=True, window=0, out=None):
+    """Attention of q [tokens, q_heads, head_dim] over the cache (`ttsamd_paged_attention`): every new token over the keys of its sequence
+    up to itself (causal) and no further back than `window` tokens, itself among them (0: all).  q_heads: a multiple of the cache's heads,
+    head h reads key head h // (q_heads // kv_heads).  scale: default head_dim ** -0.5.  A token that sees no key gets zeros; rows of
+    `out` behind the last sequence are left as they were."""
+    _need(q.dim() == 3 and q.shape[1] > 0 and q.shape[1] % cache.kv_heads == 0,
+          "q is %s: [tokens, a multiple of %d heads, head_dim] is wanted" % (tuple(q.shape), cache.kv_heads))
+    tokens, heads, dim = q.shape
+    qt, qh = _rows(q, "q", (heads, cache.head_dim), cache.dtype, cache.device)
+    _need(0 <= window < 2 ** 31, "window %d" % window)
+    ref = batch._for(cache)
+    _lib.require_gpu(q, "q")
+    o = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device) if out is None else out
+    ot, oh = _rows(o, "out", (heads, dim), cache.dtype, cache.device)
+    _need(o.shape[0] == tokens, "out has %d tokens, q %d" % (o.shape[0], tokens))
+    a = _PagedAttentionArgs(q.data_ptr(), o.data_ptr(), 0 if tokens <= 1 else qt, 0 if heads <= 1 else qh, 0 if tokens <= 1 else ot,
+                            0 if heads <= 1 else oh, tokens, heads, int(bool(causal)), int(window), dim ** -0.5 if scale is None else float(scale))
+    need = lib().ttsamd_paged_attention_workspace_bytes(ctypes.byref(a), ctypes.c_void_p(cache._ref), ref)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _queue("paged_attention", cache.device, ctypes.byref(a), ctypes.c_void_p(cache._ref), ref, P(ws), ctypes.c_size_t(need))
+    return o
+
+
+class PackedW4:
+    """A layer's 4-bit weights in the image the kernel streams (include/tts_amd.h, `ttsamd_linear_w4_args`).
+
+    qweight uint8 [n, k / 2]: two levels 0..15 a byte, the even k in the low half; scales [n, k / group] in float32, float16 or bfloat16;
+    zeros uint8 [n, k / group] or None (8 everywhere); bias [n] or None.  group = k / scales.shape[1]: 32, 64 or 128.
+    weight[n, k] = (level - zero) * scale.  Packing runs once, on the tensors' device."""
+
+    def __init__(self, qweight, scales, zeros=None, bias=None):
+        n, k = qweight.shape[0], 2 * qweight.shape[1]
+        _need(qweight.dtype == torch.uint8 and scales.dtype in _DTYPES and scales.dim() == 2 and scales.shape[0] == n and scales.shape[1] > 0,
+              "qweight uint8 [n, k / 2] and scales [n, k / group] in float32, float16 or bfloat16 are wanted")
+        group = k // scales.shape[1]
+        _need(n > 0 and group in (32, 64, 128) and group * scales.shape[1] == k, "groups of %d: 32, 64 or 128, k a multiple of it" % group)
+        _need(zeros is None or (zeros.dtype == torch.uint8 and zeros.shape == scales.shape), "zeros: uint8, shaped as the scales")
+        _need(bias is None or tuple(bias.shape) == (n,), "bias: [n]")
+        _need(all(t is None or t.device == qweight.device for t in (scales, zeros, bias)), "qweight, scales, zeros and bias are on one device")
+        tiles, chunks = -(-n // 16), -(-k // 128)
+        per = 128 // group
+        full = torch.zeros((tiles * 16, chunks * 64), dtype=torch.uint8, device=qweight.device)
+        full[:n, : k // 2] = qweight
+        words = full.view(torch.int32).view(tiles, 16, chunks, 4, 4)                     # [t, r, c, j, g]
+        self.levels = words.permute(0, 2, 4, 1, 3).contiguous()                          # [t, c, g, r, j]
+
+        def by_group(t):
+            f = torch.zeros((tiles * 16, chunks * per), dtype=t.dtype, device=t.device)
+            f[:n, : k // group] = t
+            return f.view(tiles, 16, chunks * per).transpose(1, 2).contiguous()
+
+        self.scales = by_group(scales)
+        self.zeros = None if zeros is None else by_group(zeros)
+        self.bias = bias
+        self.n, self.k, self.group, self.device = n, k, group, qweight.device
+
+    @classmethod
+    def quantize(cls, weight, group=64, bias=None, zeros=False, scale_dtype=None):
+        """The nearest levels of a [n, k] weight: symmetric (step = largest magnitude of a group / 7.5 about zero 8), or with zero points
+        (step = (max - min) / 15 of the group, zero included)."""
+        n, k = weight.shape
+        _need(k % group == 0, "k = %d is not a multiple of the group %d" % (k, group))
+        w = weight.detach().float().view(n, k // group, group)
+        if zeros:
+            lo, hi = w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)
+            step = (hi - lo) / 15
+        else:
+            step = w.abs().amax(-1) / 7.5
+        scales = step.to(scale_dtype or weight.dtype)
+        step = torch.where(scales.float() > 0, scales.float(), 1.0)[..., None]
+        zero = (-lo / step[..., 0]).round().clamp(0, 15) if zeros else torch.full_like(step[..., 0], 8)
+        q = ((w / step).round() + zero[..., None]).clamp(0, 15).to(torch.uint8).view(n, k)
+        return cls((q[:, ::2] | (q[:, 1::2] << 4)).contiguous(), scales, zero.to(torch.uint8) if zeros else None, bias)
+
+    def nbytes(self):
+        return sum(t.numel() * t.element_size() for t in (self.levels, self.scales, self.zeros, self.bias) if t is not None)
+
+
+def linear_w4(weights, x, out=None):
+    """x [rows, k] times the packed weights [n, k] transposed, plus their bias -> [rows, n] in x's type (float32, float16, bfloat16).
+    Meant for the few rows of a decoding step; any number is computed."""
+    w = weights
+    _need(x.dim() == 2 and x.shape[1] == w.k and x.dtype in _DTYPES, "x is %s %s: [rows, %d] in float32, float16 or bfloat16 is wanted"
+          % (x.dtype, tuple(x.shape), w.k))
+    _need(x.stride(1) == 1, "the channels of a row of x have to be contiguous")
+    _need(x.device == w.device and (w.bias is None or w.bias.dtype == x.dtype), "x is %s on %s, the layer %s on %s"
+          % (x.dtype, x.device, x.dtype if w.bias is None else w.bias.dtype, w.device))
+    _lib.require_gpu(x, "x")
+    m = x.shape[0]
+    y = torch.empty((m, w.n), dtype=x.dtype, device=x.device) if out is None else out
+    _need(y.shape == (m, w.n) and y.dtype == x.dtype and y.device == x.device and (w.n == 1 or y.stride(1) == 1),
+          "out: [%d, %d] %s with contiguous rows is wanted" % (m, w.n, x.dtype))
+    a = _LinearW4Args(x.data_ptr(), y.data_ptr(), x.stride(0), y.stride(0), w.levels.data_ptr(), w.scales.data_ptr(), _dp(w.zeros), _dp(w.bias),
+                      m, w.n, w.k, w.group, _DTYPES[x.dtype], _DTYPES[w.scales.dtype])
+    _queue("linear_w4", x.device, ctypes.byref(a))
+    return y
