@@ -1,108 +1,145 @@
-// Attention of new tokens over a paged key/value cache.
+// Attention of new tokens over a paged key/value cache: the choice of kernel and launch, and the entry points.
 //
 // out[t,h] = sum_j p_j v_j, p = softmax_j(scale q.k_j) over the keys token t sees, in one pass over the keys with a running maximum m
 // and sum l: a tile's scores s give m' = max(m, s), p = exp(s - m'), l = l exp(m - m') + sum p, o = o exp(m - m') + sum p v.
-// A wave per (token, query head): a lane scores one key of a tile of 64, then owns channels lane, lane + 64, .. of the output.
-#include "decode_common.h"
+#include "paged_stream.h"
 
 namespace ttsamd {
 namespace {
 
-struct AttArgs {
-    ttsamd_paged_attention_args a;
-    ttsamd_paged_kv c;
-    ttsamd_paged_batch b;
-    FastDiv by_page;
+constexpr int kCus = 256;
+
+struct Launch {
+    int dp, nq, waves, splits, split_keys, row_tiles;
+    size_t part_bytes, stat_bytes;
 };
 
-template <class T> __global__ __launch_bounds__(64) void attend_rows(AttArgs g)
+// Waves of a workgroup, by what a wave's registers allow (128, 256 or 512 of them).
+constexpr int most_waves(int dp, int nq) { return dp == 64 && nq == 1 ? 16 : dp <= 128 ? 8 : 4; }
+
+// How a call is laid over the chip.  Sizes here are hints (max_new, max_len): the kernels compute whatever the device data holds.
+Launch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv &c, const ttsamd_paged_batch &b)
 {
-    __shared__ float sq[256], sp[64];
-    __shared__ int64_t sv[64];
-    const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, blockIdx.z);
-    const int h = blockIdx.y, hk = h / (g.a.q_heads / g.c.kv_heads), lane = threadIdx.x, d = g.c.head_dim;
-    for (int i = blockIdx.x; i < s.n; i += gridDim.x) {
-        const int64_t token = s.start + i;
-        const T *q = (const T *)g.a.q + token * g.a.q_tstride + h * g.a.q_hstride;
-        __syncthreads();
-        for (int e = lane; e < d; e += 64) sq[e] = to_f(q[e]);
-        __syncthreads();
-        const int pos = s.len - s.n + i;
-        const auto [begin, end] = seen_by(s, pos, g.a.causal, g.a.window);
-        float m = -INFINITY, l = 0.f, o[4] = {};
-        for (int base = begin; base < end; base += 64) {
-            const int j = base + lane;
-            float w = -INFINITY;
-            int64_t at = -1;
-            if (j < end) {
-                int row;
-                const int64_t page = page_of(g.b, g.by_page, g.c.pages, blockIdx.z, j, row);
-                if (page >= 0) {
-                    const T *k = (const T *)g.c.k + page * g.c.k_page + hk * g.c.k_head + row * g.c.k_row;
-                    at = page * g.c.v_page + hk * g.c.v_head + row * g.c.v_row;
-                    w = 0.f;
-                    for (int e = 0; e < d; ++e) w = fmaf(sq[e], to_f(k[e]), w);
-                    w *= g.a.scale;
-                }
-            }
-            float top = w;
-            for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-            const float m2 = fmaxf(m, top);
-            const float p = at < 0 || m2 == -INFINITY ? 0.f : expf(w - m2), fade = m2 == -INFINITY ? 1.f : expf(m - m2);
-            float sum = p;
-            for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
-            l = l * fade + sum, m = m2;
-            __syncthreads();
-            sp[lane] = p, sv[lane] = at;
-            __syncthreads();
-            for (int x = 0; x < 4; ++x) o[x] *= fade;
-            for (int r = 0; r < 64; ++r) {
-                if (sv[r] < 0) continue;
-                const T *v = (const T *)g.c.v + sv[r];
-                for (int x = 0; x < 4; ++x)
-                    if (lane + 64 * x < d) o[x] = fmaf(sp[r], to_f(v[lane + 64 * x]), o[x]);
-            }
-        }
-        T *out = (T *)g.a.out + token * g.a.o_tstride + h * g.a.o_hstride;
-        for (int x = 0; x < 4; ++x)
-            if (lane + 64 * x < d) out[lane + 64 * x] = (T)(l > 0.f ? o[x] / l : l == 0.f ? 0.f : o[x] + l);
+    Launch p = {};
+    const bool f32 = c.dtype == TTSAMD_F32;
+    const int group = a.q_heads / c.kv_heads;
+    p.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
+    const int64_t rows = (int64_t)(b.max_new < 1 ? 1 : b.max_new) * group;
+    p.nq = rows > 16 && p.dp < 256 ? 2 : 1;
+    const int64_t tiles = (rows + 16 * p.nq - 1) / (16 * p.nq);
+    p.row_tiles = (int)(tiles < 65535 ? tiles : 65535);
+    const int64_t room = (int64_t)b.table_width * c.page_size;
+    int64_t keys = b.max_len > 0 && b.max_len < room ? b.max_len : room;
+    if (a.window > 0 && (int64_t)a.window + b.max_new < keys) keys = (int64_t)a.window + b.max_new;
+    const int kt = f32 || p.dp > 128 ? 16 : 32, most = most_waves(p.dp, p.nq);
+    const int64_t key_tiles = keys < 1 ? 1 : (keys + kt - 1) / kt, blocks = tiles * c.kv_heads * b.batch;
+    // Few workgroups: more waves to each, since they are joined in LDS for nothing but a barrier.
+    p.waves = 4;
+    while (p.waves < most && blocks * p.waves < kCus * 8 && key_tiles > p.waves) p.waves *= 2;
+    // Still few, and long: the keys are split over workgroups, at least four tiles to a wave, and a second launch joins them.
+    p.splits = 1;
+    const int64_t fill = (int64_t)kCus * 16 / (blocks * p.waves), long_enough = key_tiles / (p.waves * 4);
+    if (fill > 1 && long_enough > 1) p.splits = (int)(fill < long_enough ? fill : long_enough);
+    if ((int64_t)p.splits * c.kv_heads > 65535) p.splits = 65535 / c.kv_heads > 1 ? 65535 / c.kv_heads : 1;
+    const int64_t each = (key_tiles + p.splits - 1) / p.splits;
+    p.split_keys = (int)(each * kt < 0x7fffffff ? each * kt : 0x7fffffff);
+    if (p.splits > 1) {
+        const size_t n = (size_t)a.tokens * a.q_heads * p.splits;
+        p.part_bytes = n * c.head_dim * sizeof(float), p.stat_bytes = n * 2 * sizeof(float);
     }
+    return p;
 }
 
-}  // namespace
-}  // namespace ttsamd
-
-extern "C" size_t ttsamd_paged_attention_workspace_bytes(const ttsamd_paged_attention_args *, const ttsamd_paged_kv *, const ttsamd_paged_batch *)
+template <class T, int DP, int NQ, bool FULL> hipError_t start(const AttArgs &g, const Launch &p, dim3 grid, hipStream_t st)
 {
-    return 0;
+    constexpr int MAXW = most_waves(DP, NQ);
+    static std::atomic<unsigned long long> done{0};
+    const int bytes = p.waves * 16 * NQ * (DP + 4 + 2) * 4, most = MAXW * 16 * NQ * (DP + 4 + 2) * 4;
+    if (hipError_t e = ensure_dynamic_lds((const void *)attend_stream<T, DP, NQ, FULL, MAXW>, most, done)) return e;
+    attend_stream<T, DP, NQ, FULL, MAXW><<<grid, p.waves * 64, bytes, st>>>(g);
+    return hipSuccess;
+}
+template <class T, int DP, int NQ> hipError_t start(const AttArgs &g, const Launch &p, dim3 grid, hipStream_t st)
+{
+    return g.c.head_dim == DP ? start<T, DP, NQ, true>(g, p, grid, st) : start<T, DP, NQ, false>(g, p, grid, st);
+}
+template <class T> hipError_t start(const AttArgs &g, const Launch &p, hipStream_t st)
+{
+    const dim3 grid(g.c.kv_heads * p.splits, p.row_tiles, g.b.batch);
+    if (p.dp == 64) return p.nq == 2 ? start<T, 64, 2>(g, p, grid, st) : start<T, 64, 1>(g, p, grid, st);
+    if (p.dp == 128) return p.nq == 2 ? start<T, 128, 2>(g, p, grid, st) : start<T, 128, 1>(g, p, grid, st);
+    return start<T, 256, 1>(g, p, grid, st);
+}
+template <class T> void join(const AttArgs &g, hipStream_t st)
+{
+    const int64_t items = (int64_t)(g.b.max_new < 1 ? 1 : g.b.max_new) * g.a.q_heads * (g.c.head_dim / 8), blocks = (items + 255) / 256;
+    join_splits<T><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536), g.b.batch), 256, 0, st>>>(g);
 }
 
-extern "C" int ttsamd_paged_attention(const ttsamd_paged_attention_args *a, const ttsamd_paged_kv *cache, const ttsamd_paged_batch *batch,
-                                      void *, size_t, void *stream)
+int check(const ttsamd_paged_attention_args *a, const ttsamd_paged_kv *cache, const ttsamd_paged_batch *batch)
 {
-    using namespace ttsamd;
     TTSAMD_CHECK_ARG(a, "paged_attention: arguments are NULL");
     if (int rc = check_paged_kv("paged_attention", cache)) return rc;
     if (int rc = check_paged_batch("paged_attention", batch, a->tokens)) return rc;
     TTSAMD_CHECK_ARG(a->q_heads > 0 && a->q_heads % cache->kv_heads == 0, "paged_attention: %d query heads over %d key heads", a->q_heads,
                      cache->kv_heads);
     TTSAMD_CHECK_ARG(a->window >= 0, "paged_attention: window %d", a->window);
+    if (a->q_heads > 65535 || (int64_t)a->tokens * a->q_heads > (1 << 30) || (int64_t)batch->table_width * cache->page_size > 0x7fff0000) {
+        set_error("paged_attention: %d query heads of %d tokens, tables of %d pages (up to 65535 heads, 2^30 rows, 2^31 - 2^16 positions)",
+                  a->q_heads, a->tokens, batch->table_width);
+        return TTSAMD_ERR_UNSUPPORTED;
+    }
+    // row offsets travel in 16-byte units of 32 bits
+    const int es = elem_bytes(cache->dtype);
+    if ((((int64_t)cache->pages - 1) * cache->k_page + (cache->page_size - 1) * cache->k_row) * es / 16 > 0xffffffffll ||
+        (((int64_t)cache->pages - 1) * cache->v_page + (cache->page_size - 1) * cache->v_row) * es / 16 > 0xffffffffll) {
+        set_error("paged_attention: a cache that spans over 64 GiB");
+        return TTSAMD_ERR_UNSUPPORTED;
+    }
+    return TTSAMD_OK;
+}
+
+}  // namespace
+}  // namespace ttsamd
+
+extern "C" size_t ttsamd_paged_attention_workspace_bytes(const ttsamd_paged_attention_args *a, const ttsamd_paged_kv *cache,
+                                                         const ttsamd_paged_batch *batch)
+{
+    using namespace ttsamd;
+    if (check(a, cache, batch) != TTSAMD_OK || a->tokens == 0 || batch->batch == 0) return 0;
+    const Launch p = plan_of(*a, *cache, *batch);
+    return p.part_bytes + p.stat_bytes;
+}
+
+extern "C" int ttsamd_paged_attention(const ttsamd_paged_attention_args *a, const ttsamd_paged_kv *cache, const ttsamd_paged_batch *batch,
+                                      void *workspace, size_t workspace_bytes, void *stream)
+{
+    using namespace ttsamd;
+    if (int rc = check(a, cache, batch)) return rc;
     if (a->tokens == 0 || batch->batch == 0) return TTSAMD_OK;
     TTSAMD_CHECK_ARG(a->q && a->out, "paged_attention: a tensor is NULL");
     const int per = 16 / elem_bytes(cache->dtype);
     TTSAMD_CHECK_ARG((((uintptr_t)a->q | (uintptr_t)a->out) & 15) == 0 && a->q_tstride % per == 0 && a->q_hstride % per == 0 &&
                          a->o_tstride % per == 0 && a->o_hstride % per == 0,
                      "paged_attention: q and out start and stride at multiples of 16 bytes");
-    if (a->q_heads > 65535) {
-        set_error("paged_attention: %d query heads (up to 65535)", a->q_heads);
-        return TTSAMD_ERR_UNSUPPORTED;
-    }
-    AttArgs g{*a, *cache, *batch, fast_div(cache->page_size)};
-    const dim3 grid(batch->max_new < 1 ? 1 : batch->max_new, a->q_heads, batch->batch);
+    const Launch p = plan_of(*a, *cache, *batch);
+    TTSAMD_CHECK_ARG(p.splits == 1 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= p.part_bytes + p.stat_bytes),
+                     "paged_attention: a workspace of %zu bytes at a multiple of 16 is wanted", p.part_bytes + p.stat_bytes);
+    AttArgs g = {};
+    g.a = *a, g.c = *cache, g.b = *batch;
+    g.group = a->q_heads / cache->kv_heads;
+    g.by_page = fast_div(cache->page_size), g.by_group = fast_div(g.group);
+    g.scale2 = a->scale * 1.4426950408889634f;
+    g.splits = p.splits, g.split_keys = p.split_keys;
+    g.part = (float *)workspace, g.stat = (float *)((char *)workspace + p.part_bytes);
     hipStream_t st = as_stream(stream);
-    if (cache->dtype == TTSAMD_F32) attend_rows<float><<<grid, 64, 0, st>>>(g);
-    else if (cache->dtype == TTSAMD_F16) attend_rows<_Float16><<<grid, 64, 0, st>>>(g);
-    else attend_rows<__bf16><<<grid, 64, 0, st>>>(g);
+    TTSAMD_HIP(cache->dtype == TTSAMD_F32 ? start<float>(g, p, st) : cache->dtype == TTSAMD_F16 ? start<_Float16>(g, p, st) : start<__bf16>(g, p, st));
     TTSAMD_LAUNCH_CHECK();
+    if (p.splits > 1) {
+        if (cache->dtype == TTSAMD_F32) join<float>(g, st);
+        else if (cache->dtype == TTSAMD_F16) join<_Float16>(g, st);
+        else join<__bf16>(g, st);
+        TTSAMD_LAUNCH_CHECK();
+    }
     return TTSAMD_OK;
 }

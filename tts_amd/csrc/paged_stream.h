@@ -1,0 +1,396 @@
+// Attention of few rows over a long paged cache: keys and values stream from memory through registers into the matrix unit.
+//
+// Rows.  All query heads that read one key head, of all new tokens of a sequence, are rows of one problem: row r = token r / G,
+// head r % G (G = q_heads / kv_heads).  A workgroup takes NQ tiles of 16 rows; its waves take the tiles of its keys in turn, each with
+// a running maximum and sum of its own, and are joined in LDS at the end.
+//
+// Layout.  S^T = K Q^T is computed with the keys as the matrix rows, so that in the 16x16 result a lane holds one query row (column
+// lane % 16) and the keys 4 (lane / 16) + i: maximum, exponential and sum stay in the lane.  The same registers, rounded to T, are the
+// right operand of O^T = V^T P^T as they lie, because the order of the keys inside a contraction is free: slot (lane / 16, e) of the
+// 32-deep product is key 4 (lane / 16) + e of the first 16 keys for e < 4, of the second for e >= 4.  The left operand V^T wants, per
+// lane, eight keys of one channel; a lane loads eight keys of NV = DP / 16 neighbouring channels (16 bytes and whole lines at DP = 128)
+// and regroups the halves with one v_perm per pair, so nothing passes through LDS.  fp32 uses the 4-deep fp32 product: no regrouping,
+// 16 keys a tile.
+//
+// The running maximum moves only when a score exceeds it by more than 2^8 (p <= 256 then, exact in every type's range): the cross-lane
+// maximum and the scaling of O are skipped in almost every tile.
+//
+// Where a tile's rows lie (page lookup, one key a lane, keys in lanes 0-31 and values in lanes 32-63) is fetched a tile ahead; a
+// key without a place gets the cache's first row and is masked, its value zeroed, so no lane ever reads outside the pages.
+//
+// A value that is an infinity or NaN must not reach rows that do not see its key, and 0 * infinity would: where a tile is seen by some
+// rows only and holds such a value, the rows are computed again key by key.
+//
+// Bound: HBM for single tokens.
+#pragma once
+#include "decode_common.h"
+
+namespace ttsamd {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+constexpr float kNoMax = -1e38f;     // a running maximum before the first key: finite, so that no difference of two is NaN
+constexpr float kLazy = 8.f;         // how far (log2) a score may exceed the running maximum before it moves
+
+struct AttArgs {
+    ttsamd_paged_attention_args a;
+    ttsamd_paged_kv c;
+    ttsamd_paged_batch b;
+    FastDiv by_page, by_group;       // group = query heads a key head
+    float scale2;                    // scale * log2 e
+    int group, splits, split_keys;   // split_keys: keys of a split (the last takes the rest)
+    float *part;                     // splits > 1: [tokens * q_heads][splits][head_dim], then [tokens * q_heads][splits][2]
+    float *stat;
+};
+
+template <class T> __device__ __forceinline__ f32x4_t mfma_16x16x32(uint4 a, uint4 b, f32x4_t c);
+template <> __device__ __forceinline__ f32x4_t mfma_16x16x32<__bf16>(uint4 a, uint4 b, f32x4_t c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x4_t mfma_16x16x32<_Float16>(uint4 a, uint4 b, f32x4_t c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+template <class T> __device__ __forceinline__ f32x4_t mfma_16x16x16(uint2 a, uint2 b, f32x4_t c)
+{
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4, a), __builtin_bit_cast(s4, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(h4, a), __builtin_bit_cast(h4, b), c, 0, 0, 0);
+}
+template <class T> __device__ __forceinline__ unsigned pack2(float x, float y)
+{
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f2{x, y}), t2));
+}
+// Whether a 32-bit word of T holds an infinity or NaN.
+template <class T> __device__ __forceinline__ bool any_odd(unsigned w)
+{
+    constexpr unsigned X = __is_same(T, float) ? 0x7f800000u : __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
+    if constexpr (sizeof(T) == 4) return (w & X) == X;
+    else return (w & X) == X || (w >> 16 & X) == X;
+}
+
+// One row's keys [lo, hi), a wave, key by key: o[d] += p v only for the keys of `see`.  For the rare tile where a value that some row
+// must not see is an infinity or NaN.
+template <class T>
+__device__ void attend_row(const AttArgs &g, int b, int hk, const T *q, Range see, float *o, float *ml)
+{
+    const int lane = threadIdx.x & 63, D = g.c.head_dim;
+    float m = kNoMax, l = 0.f, acc[4] = {};
+    for (int j = see.begin; j < see.end; ++j) {
+        int row;
+        const int64_t page = page_of(g.b, g.by_page, g.c.pages, b, j, row);
+        if (page < 0) continue;
+        const T *k = (const T *)g.c.k + page * g.c.k_page + hk * g.c.k_head + row * g.c.k_row;
+        const T *v = (const T *)g.c.v + page * g.c.v_page + hk * g.c.v_head + row * g.c.v_row;
+        float x = 0.f;
+        for (int d = lane; d < D; d += 64) x = fmaf(to_f(q[d]), to_f(k[d]), x);
+        for (int y = 32; y; y >>= 1) x += __shfl_xor(x, y);
+        const float to = fmaxf(m, x * g.scale2), fade = __builtin_amdgcn_exp2f(m - to), p = __builtin_amdgcn_exp2f(fmaf(x, g.scale2, -to));
+        m = to, l = l * fade + p;
+        for (int y = 0; y < 4; ++y)
+            if (lane + 64 * y < D) acc[y] = fmaf(p, to_f(v[lane + 64 * y]), acc[y] * fade);
+    }
+    for (int y = 0; y < 4; ++y)
+        if (lane + 64 * y < D) o[lane + 64 * y] = acc[y];
+    if (lane == 0) ml[0] = m, ml[1] = l;
+}
+
+template <class T, int DP, int NQ, bool FULL, int MAXW>
+__global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
+{
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int ES = sizeof(T), RB = DP * ES, NS = RB / 64, NV = DP / 16, KT = F32 || DP > 128 ? 16 : 32, NT = KT / 16;
+    constexpr int VK = KT / 4;                          // values (keys) a lane holds of a tile
+    constexpr int VB = NV * ES, VP = VB < 16 ? 8 : 16;  // bytes of a lane's channels of one key, and of one load
+    extern __shared__ float lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int c16 = lane & 15, g4 = lane >> 4;
+    const int hk = blockIdx.x / g.splits, split = blockIdx.x - hk * g.splits, b = blockIdx.z;
+    const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, b);
+    const int D = g.c.head_dim, rows = s.n * g.group;
+    const char *kbase = (const char *)g.c.k + (int64_t)hk * g.c.k_head * ES, *vbase = (const char *)g.c.v + (int64_t)hk * g.c.v_head * ES;
+    const bool vrole = lane >= 32;
+    const uint32_t page16 = (uint32_t)((vrole ? g.c.v_page : g.c.k_page) * ES / 16), row16 = (uint32_t)((vrole ? g.c.v_row : g.c.k_row) * ES / 16);
+
+    for (int r0 = blockIdx.y * 16 * NQ; r0 < rows; r0 += gridDim.y * 16 * NQ) {
+        const int last = min(r0 + 16 * NQ, rows) - 1;
+        Range mine[NQ];
+        uint4 q[NQ][NS];
+#pragma unroll
+        for (int u = 0; u < NQ; ++u) {
+            const int r = min(r0 + 16 * u + c16, last), i = g.by_group.div(r), h = hk * g.group + r - i * g.group;
+            mine[u] = seen_by(s, s.len - s.n + i, g.a.causal, g.a.window);
+            const char *src = (const char *)g.a.q + ((int64_t)(s.start + i) * g.a.q_tstride + (int64_t)h * g.a.q_hstride) * ES;
+#pragma unroll
+            for (int x = 0; x < NS; ++x) {
+                const int at = x * 64 + g4 * 16;
+                q[u][x] = FULL || at < D * ES ? *(const uint4 *)(src + (FULL || at < D * ES ? at : 0)) : uint4{0, 0, 0, 0};
+            }
+        }
+        const Range first = seen_by(s, s.len - s.n + (int)g.by_group.div(r0), g.a.causal, g.a.window);
+        const Range final = seen_by(s, s.len - s.n + (int)g.by_group.div(last), g.a.causal, g.a.window);
+        // ranges move to the right with the row: the union is [first.begin, final.end), the intersection [final.begin, first.end)
+        const int64_t from = first.begin + (int64_t)split * g.split_keys, to = split + 1 < g.splits ? from + g.split_keys : final.end;
+        const int lo = (int)min(from, (int64_t)final.end), hi = (int)min(to, (int64_t)final.end);
+
+        f32x4_t o[NQ][NV];
+        float m[NQ], l[NQ];
+#pragma unroll
+        for (int u = 0; u < NQ; ++u) {
+            m[u] = kNoMax, l[u] = 0.f;
+#pragma unroll
+            for (int x = 0; x < NV; ++x) o[u][x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+
+        bool odd = false;
+        int base = lo + wave * KT;
+        const int step = waves * KT, idx = lane & (KT - 1);
+        uint4 k[NT][NS];
+        unsigned v[VK][VB / 4];
+        // place of this lane's key of the tile at `at`: the table's page, -1 where the key is not one of [lo, hi)
+        auto fetch = [&](int at, int &row) {
+            const int j = at + idx;
+            row = 0;
+            return j < hi ? page_of(g.b, g.by_page, g.c.pages, b, j, row) : -1;
+        };
+        auto load_k = [&](uint32_t off) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const char *p = kbase + (uint64_t)(uint32_t)__shfl((int)off, 16 * t + c16) * 16;
+#pragma unroll
+                for (int x = 0; x < NS; ++x) {
+                    const int at = x * 64 + g4 * 16;
+                    k[t][x] = *(const uint4 *)(p + (FULL || at < D * ES ? at : 0));
+                    if (!FULL && at >= D * ES) k[t][x] = uint4{0, 0, 0, 0};
+                }
+            }
+        };
+        int row_next = 0, page_next = -1;
+        uint32_t off = 0;
+        unsigned ok = 0;
+        if (base < hi) {
+            int row;
+            const int page = fetch(base, row);
+            off = page < 0 ? 0 : (uint32_t)page * page16 + (uint32_t)row * row16;
+            ok = (unsigned)__ballot(page >= 0) & (KT == 32 ? ~0u : 0xffffu);
+            load_k(off);
+            page_next = fetch(base + step, row_next);
+        }
+        for (; base < hi; base += step) {
+            // values of this tile: slot e of lane group g4 is key 4 g4 + e (e < 4), 16 + 4 g4 + e - 4
+#pragma unroll
+            for (int e = 0; e < VK; ++e) {
+                const char *p = vbase + (uint64_t)(uint32_t)__shfl((int)off, 32 + (e & 3) + 4 * g4 + (e >> 2) * 16) * 16;
+#pragma unroll
+                for (int x = 0; x < VB / VP; ++x) {
+                    const int at = c16 * VB + x * VP, in = FULL || at < D * ES ? at : 0;
+                    if constexpr (VP == 8) {
+                        const uint2 w = *(const uint2 *)(p + in);
+                        v[e][0] = w.x, v[e][1] = w.y;
+                    } else {
+                        const uint4 w = *(const uint4 *)(p + in);
+                        v[e][4 * x] = w.x, v[e][4 * x + 1] = w.y, v[e][4 * x + 2] = w.z, v[e][4 * x + 3] = w.w;
+                    }
+                }
+            }
+            const unsigned ok_now = ok;
+            off = page_next < 0 ? 0 : (uint32_t)page_next * page16 + (uint32_t)row_next * row16;
+            ok = (unsigned)__ballot(page_next >= 0) & (KT == 32 ? ~0u : 0xffffu);
+            page_next = fetch(base + 2 * step, row_next);
+
+            f32x4_t sc[NQ][NT];
+#pragma unroll
+            for (int u = 0; u < NQ; ++u)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int x = 0; x < NS; ++x) {
+                        if constexpr (F32) {
+                            const f32x4_t kk = __builtin_bit_cast(f32x4_t, k[t][x]), qq = __builtin_bit_cast(f32x4_t, q[u][x]);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[j], qq[j], acc, 0, 0, 0);
+                        } else {
+                            acc = mfma_16x16x32<T>(k[t][x], q[u][x], acc);
+                        }
+                    }
+                    sc[u][t] = acc;
+                }
+            if (base + step < hi) load_k(off);
+
+            const bool clear = ok_now == (KT == 32 ? ~0u : 0xffffu) && base >= final.begin && base + KT <= first.end;
+            if (!clear) {
+#pragma unroll
+                for (int e = 0; e < VK; ++e) {
+                    const bool held = ok_now >> ((e & 3) + 4 * g4 + (e >> 2) * 16) & 1;
+#pragma unroll
+                    for (int x = 0; x < VB / 4; ++x) {
+                        if (!held) v[e][x] = 0;                              // 0 * p stays 0 whatever lies there
+                        else if (s.n > 1) odd |= any_odd<T>(v[e][x]);        // 0 * infinity would not
+                    }
+                }
+            }
+            float p[NQ][VK];
+#pragma unroll
+            for (int u = 0; u < NQ; ++u) {
+                unsigned dark = 0;                           // slots that this row does not see
+                if (!clear) {
+#pragma unroll
+                    for (int e = 0; e < VK; ++e) {
+                        const int kk = (e & 3) + 4 * g4 + (e >> 2) * 16, j = base + kk;
+                        if (!(ok_now >> kk & 1) || j < mine[u].begin || j >= mine[u].end) dark |= 1u << e;
+                    }
+                }
+                float top = kNoMax;
+#pragma unroll
+                for (int e = 0; e < VK; ++e) top = fmaxf(top, !clear && (dark >> e & 1) ? kNoMax : sc[u][e >> 2][e & 3] * g.scale2);
+                if (__any(top > m[u] + kLazy)) {
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const float to = fmaxf(m[u], top), fade = __builtin_amdgcn_exp2f(m[u] - to);
+                    m[u] = to, l[u] *= fade;
+#pragma unroll
+                    for (int x = 0; x < NV; ++x) o[u][x] *= fade;
+                }
+#pragma unroll
+                for (int e = 0; e < VK; ++e) {
+                    p[u][e] = __builtin_amdgcn_exp2f(fmaf(sc[u][e >> 2][e & 3], g.scale2, -m[u]));
+                    if (!clear && (dark >> e & 1)) p[u][e] = 0.f;
+                    l[u] += p[u][e];
+                }
+            }
+            if constexpr (F32) {
+#pragma unroll
+                for (int e = 0; e < VK; ++e)
+#pragma unroll
+                    for (int x = 0; x < NV; ++x)
+#pragma unroll
+                        for (int u = 0; u < NQ; ++u)
+                            o[u][x] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[e][x]), p[u][e], o[u][x], 0, 0, 0);
+            } else if constexpr (KT == 16) {
+                uint2 pb[NQ];
+#pragma unroll
+                for (int u = 0; u < NQ; ++u) pb[u] = uint2{pack2<T>(p[u][0], p[u][1]), pack2<T>(p[u][2], p[u][3])};
+#pragma unroll
+                for (int x = 0; x < NV; ++x) {
+                    const unsigned sel = x & 1 ? 0x07060302u : 0x05040100u;
+                    const uint2 vt = {__builtin_amdgcn_perm(v[1][x / 2], v[0][x / 2], sel), __builtin_amdgcn_perm(v[3][x / 2], v[2][x / 2], sel)};
+#pragma unroll
+                    for (int u = 0; u < NQ; ++u) o[u][x] = mfma_16x16x16<T>(vt, pb[u], o[u][x]);
+                }
+            } else {
+                uint4 pb[NQ];
+#pragma unroll
+                for (int u = 0; u < NQ; ++u)
+                    pb[u] = uint4{pack2<T>(p[u][0], p[u][1]), pack2<T>(p[u][2], p[u][3]), pack2<T>(p[u][4], p[u][5]), pack2<T>(p[u][6], p[u][7])};
+#pragma unroll
+                for (int x = 0; x < NV; ++x) {
+                    const unsigned sel = x & 1 ? 0x07060302u : 0x05040100u;
+                    const uint4 vt = {__builtin_amdgcn_perm(v[1][x / 2], v[0][x / 2], sel), __builtin_amdgcn_perm(v[3][x / 2], v[2][x / 2], sel),
+                                      __builtin_amdgcn_perm(v[5][x / 2], v[4][x / 2], sel), __builtin_amdgcn_perm(v[7][x / 2], v[6][x / 2], sel)};
+#pragma unroll
+                    for (int u = 0; u < NQ; ++u) o[u][x] = mfma_16x16x32<T>(vt, pb[u], o[u][x]);
+                }
+            }
+        }
+
+        // join the waves: o [wave][row][DP + 4], then m, l [wave][row]
+        constexpr int R = 16 * NQ, LDO = DP + 4;
+        float *const ml = lds + waves * R * LDO;
+        const bool redo = __syncthreads_or(odd);            // and the last row tile's readers are done
+        if (redo) {
+            for (int r = r0 + wave; r <= last; r += waves) {
+                const int i = g.by_group.div(r), h = hk * g.group + r - i * g.group;
+                Range see = seen_by(s, s.len - s.n + i, g.a.causal, g.a.window);
+                see.begin = max(see.begin, lo), see.end = min(see.end, hi);
+                attend_row<T>(g, b, hk, (const T *)g.a.q + (int64_t)(s.start + i) * g.a.q_tstride + (int64_t)h * g.a.q_hstride, see,
+                              lds + (r - r0) * LDO, ml + 2 * (r - r0));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < NQ; ++u) {
+            l[u] += __shfl_xor(l[u], 16);
+            l[u] += __shfl_xor(l[u], 32);
+            const int row = wave * R + 16 * u + c16;
+            if (!redo && r0 + 16 * u + c16 <= last) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int x = 0; x < NV; x += 4)
+                        *(f32x4_t *)(lds + row * LDO + NV * (4 * g4 + i) + x) = f32x4_t{o[u][x][i], o[u][x + 1][i], o[u][x + 2][i], o[u][x + 3][i]};
+                if (g4 == 0) ml[2 * row] = m[u], ml[2 * row + 1] = l[u];
+            }
+        }
+        __syncthreads();
+        const int cols = D / 8, nr = last - r0 + 1;
+        for (int w = threadIdx.x; w < nr * cols; w += blockDim.x) {
+            const int r = w / cols, d = (w - r * cols) * 8;
+            float top = kNoMax, sum = 0.f, acc[8] = {};
+            const int parts = redo ? 1 : waves;
+            for (int x = 0; x < parts; ++x) top = fmaxf(top, ml[2 * (x * R + r)]);
+            for (int x = 0; x < parts; ++x) {
+                const float f = __builtin_amdgcn_exp2f(ml[2 * (x * R + r)] - top);
+                sum += f * ml[2 * (x * R + r) + 1];
+                const float *src = lds + (x * R + r) * LDO + d;
+#pragma unroll
+                for (int y = 0; y < 8; ++y) acc[y] = fmaf(f, src[y], acc[y]);
+            }
+            const int row = r0 + r, i = g.by_group.div(row), h = hk * g.group + row - i * g.group;
+            const int64_t token = s.start + i;
+            if (g.splits > 1) {
+                const int64_t at = (token * g.a.q_heads + h) * g.splits + split;
+                *(f32x4_t *)(g.part + at * D + d) = f32x4_t{acc[0], acc[1], acc[2], acc[3]};
+                *(f32x4_t *)(g.part + at * D + d + 4) = f32x4_t{acc[4], acc[5], acc[6], acc[7]};
+                if (d == 0) g.stat[2 * at] = top, g.stat[2 * at + 1] = sum;
+            } else {
+                alignas(16) T out[8];
+                const float inv = sum > 0.f ? 1.f / sum : sum;          // no key: zeros; NaN stays
+#pragma unroll
+                for (int y = 0; y < 8; ++y) out[y] = (T)(acc[y] * inv);
+                T *dst = (T *)g.a.out + token * g.a.o_tstride + (int64_t)h * g.a.o_hstride + d;
+#pragma unroll
+                for (int y = 0; y < 8 * ES / 16; ++y) ((uint4 *)dst)[y] = ((const uint4 *)out)[y];
+            }
+        }
+    }
+}
+
+// Joins the splits of every row: 8 channels a thread.
+template <class T> __global__ __launch_bounds__(256) void join_splits(AttArgs g)
+{
+    constexpr int ES = sizeof(T);
+    const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, blockIdx.y);
+    const int D = g.c.head_dim, cols = D / 8, items = g.a.q_heads * cols;
+    for (int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x; w < (int64_t)s.n * items; w += (int64_t)gridDim.x * 256) {
+        const int64_t row = w / cols;                     // (token of the sequence, head)
+        const int d = (int)(w - row * cols) * 8;
+        const int64_t at = ((int64_t)s.start * g.a.q_heads + row) * g.splits;
+        float top = kNoMax, sum = 0.f, acc[8] = {};
+        for (int x = 0; x < g.splits; ++x) top = fmaxf(top, g.stat[2 * (at + x)]);
+        for (int x = 0; x < g.splits; ++x) {
+            const float f = __builtin_amdgcn_exp2f(g.stat[2 * (at + x)] - top);
+            sum += f * g.stat[2 * (at + x) + 1];
+            const f32x4_t a0 = *(const f32x4_t *)(g.part + (at + x) * D + d), a1 = *(const f32x4_t *)(g.part + (at + x) * D + d + 4);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) acc[y] = fmaf(f, a0[y], acc[y]), acc[4 + y] = fmaf(f, a1[y], acc[4 + y]);
+        }
+        alignas(16) T out[8];
+        const float inv = sum > 0.f ? 1.f / sum : sum;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) out[y] = (T)(acc[y] * inv);
+        const int64_t token = s.start + row / g.a.q_heads;
+        const int h = (int)(row % g.a.q_heads);
+        T *dst = (T *)g.a.out + token * g.a.o_tstride + (int64_t)h * g.a.o_hstride + d;
+#pragma unroll
+        for (int y = 0; y < 8 * ES / 16; ++y) ((uint4 *)dst)[y] = ((const uint4 *)out)[y];
+    }
+}
+
+}  // namespace ttsamd
