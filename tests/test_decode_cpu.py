@@ -176,7 +176,7 @@ def test_w4_image_holds_every_level_in_its_place():
     for i in range(32):
         for j in range(256):
             word = int(pw.levels[i // 16, j // 128, j % 32 // 8, i % 16, j % 128 // 32]) & 0xFFFFFFFF
-            assert (word >> (4 * (j % 8))) & 15 == (level(i, j) if i < n and j < k else 0)
+            assert (word >> (4 * (j % 8 // 2) + 16 * (j % 2))) & 15 == (level(i, j) if i < n and j < k else 0)
             if j % group == 0:
                 inside = i < n and j < k
                 assert float(pw.scales[i // 16, j // group, i % 16]) == (float(s[i, j // group]) if inside else 0.0)

@@ -1088,7 +1088,10 @@ class PackedW4:
         per = 128 // group
         full = torch.zeros((tiles * 16, chunks * 64), dtype=torch.uint8, device=qweight.device)
         full[:n, : k // 2] = qweight
-        words = full.view(torch.int32).view(tiles, 16, chunks, 4, 4)                     # [t, r, c, j, g]
+        # of eight levels 0 .. 7 in four bytes, the even ones go to the lower half of the word, the odd ones to the upper
+        b = full.view(-1, 2, 2)
+        full = torch.stack([b[..., 0] & 15 | b[..., 1] << 4, b[..., 0] >> 4 | b[..., 1] & 240], 1).contiguous()
+        words = full.view(-1).view(torch.int32).view(tiles, 16, chunks, 4, 4)                     # [t, r, c, j, g]
         self.levels = words.permute(0, 2, 4, 1, 3).contiguous()                          # [t, c, g, r, j]
 
         def by_group(t):
