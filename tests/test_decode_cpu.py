@@ -38,6 +38,11 @@ def test_structs_match_the_header(tmp_path):
     lines = subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.strip().splitlines()
     for (name, s), line in zip(pairs, lines):
         assert [int(v) for v in line.split()] == [getattr(s, f).offset for f, _ in s._fields_] + [ctypes.sizeof(s)], name
+    # the packed forms of the per-call structs are those mirrors' bytes
+    for pack, s in ((ops._PACK_ROTARY, ops._RotaryArgs), (ops._PACK_APPEND, ops._KvAppendArgs), (ops._PACK_ATTENTION, ops._PagedAttentionArgs),
+                    (ops._PACK_W4, ops._LinearW4Args)):
+        values = [0.5 if t is ctypes.c_float else 1000 + i for i, (_, t) in enumerate(s._fields_)]
+        assert pack(*values) == bytes(s(*values)), s
 
 
 @pytest.mark.parametrize("rd,kw", [(64, {}), (32, {"scaling": {"kind": "linear", "factor": 4.0}}), (128, {"scaling": {"kind": "base", "factor": 8.0}}),

@@ -159,14 +159,14 @@ template <class T, int MT, int NT, int GROUP, int MAXW> __global__ __launch_boun
 template <class T, int MT, int NT, int GROUP> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
 {
     constexpr int MAXW = MT == 1 ? 16 : 8;
-    const int chunks = (a.k + 127) / 128, blocks = (a.n + 16 * NT - 1) / (16 * NT);
+    const int chunks = (a.k + 127) / 128, blocks = (a.n + 16 * NT - 1) / (16 * NT), row_blocks = (a.m + 16 * MT - 1) / (16 * MT);
     // Waves share the chunks of k: eight, or sixteen where there are fewer workgroups than compute units.
-    int waves = MAXW > 8 && blocks < 256 ? 16 : 8;
+    int waves = MAXW > 8 && blocks * row_blocks < 256 ? 16 : 8;
     while (waves > 1 && waves > chunks) waves /= 2;
     const int rows = a.m < 16 * MT ? a.m : 16 * MT, bytes = waves * rows * (16 * NT + 1) * 4;
     static std::atomic<unsigned long long> done{0};
     if (hipError_t e = ensure_dynamic_lds((const void *)linear_w4<T, MT, NT, GROUP, MAXW>, MAXW * 16 * MT * (16 * NT + 1) * 4, done)) return e;
-    linear_w4<T, MT, NT, GROUP, MAXW><<<dim3(blocks, (a.m + 16 * MT - 1) / (16 * MT)), waves * 64, bytes, st>>>(a);
+    linear_w4<T, MT, NT, GROUP, MAXW><<<dim3(blocks, row_blocks), waves * 64, bytes, st>>>(a);
     return hipSuccess;
 }
 template <class T, int MT, int NT> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
@@ -179,7 +179,11 @@ template <class T, int MT> hipError_t start(const ttsamd_linear_w4_args &a, hipS
 }
 template <class T> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
 {
-    return a.m <= 16 ? start<T, 1>(a, st) : a.m <= 32 ? start<T, 2>(a, st) : start<T, 4>(a, st);
+    // Rows beyond 16 share the unpacked weights where the output tiles alone fill the chip; else they are workgroups of their own,
+    // which read the weights again from the cache.
+    const int tiles = (a.n + 15) / 16;
+    if (a.m <= 16 || tiles * ((a.m + 15) / 16) <= 512) return start<T, 1>(a, st);
+    return a.m <= 32 || tiles * ((a.m + 31) / 32) <= 512 ? start<T, 2>(a, st) : start<T, 4>(a, st);
 }
 
 }  // namespace

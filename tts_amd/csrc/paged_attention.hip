@@ -72,8 +72,8 @@ template <class T> hipError_t start(const AttArgs &g, const Launch &p, hipStream
 }
 template <class T> void join(const AttArgs &g, hipStream_t st)
 {
-    const int64_t items = (int64_t)(g.b.max_new < 1 ? 1 : g.b.max_new) * g.a.q_heads * (g.c.head_dim / 8), blocks = (items + 255) / 256;
-    join_splits<T><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536), g.b.batch), 256, 0, st>>>(g);
+    const int n = g.b.max_new < 1 ? 1 : g.b.max_new;
+    join_splits<T><<<dim3(n < 65536 ? n : 65536, g.a.q_heads, g.b.batch), 256, 0, st>>>(g);
 }
 
 int check(const ttsamd_paged_attention_args *a, const ttsamd_paged_kv *cache, const ttsamd_paged_batch *batch)

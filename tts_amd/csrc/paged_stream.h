@@ -362,34 +362,53 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
     }
 }
 
-// Joins the splits of every row: 8 channels a thread.
+// Joins the splits of one (token, head): a thread owns eight channels of every 256 / (head_dim / 8)-th split, LDS adds them up.
 template <class T> __global__ __launch_bounds__(256) void join_splits(AttArgs g)
 {
     constexpr int ES = sizeof(T);
-    const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, blockIdx.y);
-    const int D = g.c.head_dim, cols = D / 8, items = g.a.q_heads * cols;
-    for (int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x; w < (int64_t)s.n * items; w += (int64_t)gridDim.x * 256) {
-        const int64_t row = w / cols;                     // (token of the sequence, head)
-        const int d = (int)(w - row * cols) * 8;
-        const int64_t at = ((int64_t)s.start * g.a.q_heads + row) * g.splits;
+    __shared__ float lds[256 * 9];
+    const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, blockIdx.z);
+    const int D = g.c.head_dim, cols = D / 8, lanes = 256 / cols, h = blockIdx.y;
+    const int at_col = threadIdx.x % cols, at_lane = threadIdx.x / cols, d = at_col * 8;
+    for (int i = blockIdx.x; i < s.n; i += gridDim.x) {
+        const int64_t token = s.start + i, at = (token * g.a.q_heads + h) * g.splits;
         float top = kNoMax, sum = 0.f, acc[8] = {};
-        for (int x = 0; x < g.splits; ++x) top = fmaxf(top, g.stat[2 * (at + x)]);
-        for (int x = 0; x < g.splits; ++x) {
-            const float f = __builtin_amdgcn_exp2f(g.stat[2 * (at + x)] - top);
-            sum += f * g.stat[2 * (at + x) + 1];
-            const f32x4_t a0 = *(const f32x4_t *)(g.part + (at + x) * D + d), a1 = *(const f32x4_t *)(g.part + (at + x) * D + d + 4);
+        if (at_lane < lanes) {
+            for (int x = at_lane; x < g.splits; x += lanes) top = fmaxf(top, g.stat[2 * (at + x)]);
+            for (int x = at_lane; x < g.splits; x += lanes) {
+                const float f = __builtin_amdgcn_exp2f(g.stat[2 * (at + x)] - top);
+                sum += f * g.stat[2 * (at + x) + 1];
+                const f32x4_t a0 = *(const f32x4_t *)(g.part + (at + x) * D + d), a1 = *(const f32x4_t *)(g.part + (at + x) * D + d + 4);
 #pragma unroll
-            for (int y = 0; y < 4; ++y) acc[y] = fmaf(f, a0[y], acc[y]), acc[4 + y] = fmaf(f, a1[y], acc[4 + y]);
+                for (int y = 0; y < 4; ++y) acc[y] = fmaf(f, a0[y], acc[y]), acc[4 + y] = fmaf(f, a1[y], acc[4 + y]);
+            }
         }
-        alignas(16) T out[8];
-        const float inv = sum > 0.f ? 1.f / sum : sum;
+        // each has a maximum of its own: brought to the largest, then added in the order of the lanes
+        float *const mine = lds + threadIdx.x * 9;
+        __syncthreads();
+        mine[8] = top;
+        __syncthreads();
+        float best = top;
+        for (int x = 0; x < lanes; ++x) best = fmaxf(best, lds[(x * cols + at_col) * 9 + 8]);
+        const float f = __builtin_amdgcn_exp2f(top - best);
+        __syncthreads();
 #pragma unroll
-        for (int y = 0; y < 8; ++y) out[y] = (T)(acc[y] * inv);
-        const int64_t token = s.start + row / g.a.q_heads;
-        const int h = (int)(row % g.a.q_heads);
-        T *dst = (T *)g.a.out + token * g.a.o_tstride + (int64_t)h * g.a.o_hstride + d;
+        for (int y = 0; y < 8; ++y) mine[y] = acc[y] * f;
+        mine[8] = sum * f;
+        __syncthreads();
+        if (at_lane == 0) {
+            float all[9] = {};
+            for (int x = 0; x < lanes; ++x)
 #pragma unroll
-        for (int y = 0; y < 8 * ES / 16; ++y) ((uint4 *)dst)[y] = ((const uint4 *)out)[y];
+                for (int y = 0; y < 9; ++y) all[y] += lds[(x * cols + at_col) * 9 + y];
+            alignas(16) T out[8];
+            const float inv = all[8] > 0.f ? 1.f / all[8] : all[8];
+#pragma unroll
+            for (int y = 0; y < 8; ++y) out[y] = (T)(all[y] * inv);
+            T *dst = (T *)g.a.out + token * g.a.o_tstride + (int64_t)h * g.a.o_hstride + d;
+#pragma unroll
+            for (int y = 0; y < 8 * ES / 16; ++y) ((uint4 *)dst)[y] = ((const uint4 *)out)[y];
+        }
     }
 }
 

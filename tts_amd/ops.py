@@ -6,6 +6,7 @@ re-ordering, MFMA fragment packing) runs once at load time.
 """
 import ctypes
 import os
+import struct
 import threading
 import time
 
@@ -840,11 +841,21 @@ class _LinearW4Args(ctypes.Structure):
         [(n, ctypes.c_int32) for n in ("m", "n", "k", "group", "dtype", "scale_dtype")]
 
 
+def _refuse(message):
+    raise _lib.TtsAmdError(message)
+
+
 def _need(ok, message):
     if not ok:
-        raise _lib.TtsAmdError(message)
+        _refuse(message)
 
 
+# The structs of the per-call arguments, packed as C lays them out (the ctypes mirrors above spell the fields; a step of a small model
+# is mostly these calls, and packing a struct of a dozen fields takes a fifth of filling its mirror).
+_PACK_ROTARY = struct.Struct("PPqqqqPiiiiii0q").pack
+_PACK_APPEND = struct.Struct("PPqqqqPPqqqqPiii0q").pack
+_PACK_ATTENTION = struct.Struct("PPqqqqiiiif0q").pack
+_PACK_W4 = struct.Struct("PPqqPPPPiiiiii0q").pack
 _FNS = {}
 
 
@@ -852,23 +863,28 @@ def _queue(what, device, *args):
     """One call of the library's function `what` on the current stream of `device` (made current for the call if it is not)."""
     fn = _FNS.get(what)
     if fn is None:
-        fn = _FNS[what] = getattr(lib(), "ttsamd_" + what)
+        fn = getattr(lib(), "ttsamd_" + what)
+        fn.argtypes = [ctypes.c_char_p] + [ctypes.c_void_p] * (len(args) - 1) + [ctypes.c_void_p]
+        _FNS[what] = fn
     index = device.index
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
             return _queue(what, device, *args)
-    rc = fn(*args, ctypes.c_void_p(torch.cuda.current_stream(index).cuda_stream))
+    rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         check(rc, what)
 
 
-def _rows(t, what, heads_dim, dtype, device):
-    """A [tokens, heads, head_dim] tensor of the call: checked, its (token, head) strides returned."""
-    _need(t.dim() == 3 and t.shape[1:] == heads_dim, "%s is %s: [tokens, %d, %d] is wanted" % (what, tuple(t.shape), *heads_dim))
-    _need(t.dtype == dtype and t.device == device, "%s is %s on %s: %s on %s is wanted" % (what, t.dtype, t.device, dtype, device))
+def _rows(t, what, shape, dtype, device):
+    """A [tokens, heads, head_dim] tensor of the call, checked against `shape`; its (token, head) strides, 0 where there is one entry."""
+    if t.shape != shape:
+        _refuse("%s is %s: %s is wanted" % (what, list(t.shape), list(shape)))
+    if t.dtype != dtype or t.device != device:
+        _refuse("%s is %s on %s: %s on %s is wanted" % (what, t.dtype, t.device, dtype, device))
     st, sh, sd = t.stride()
-    _need(sd == 1 or t.shape[2] <= 1, "%s: the channels of a head have to be contiguous" % what)
-    return st, sh
+    if sd != 1 and shape[2] > 1:
+        _refuse("%s: the channels of a head have to be contiguous" % what)
+    return st if shape[0] > 1 else 0, sh if shape[1] > 1 else 0
 
 
 def _inner(s, shape):
@@ -932,28 +948,32 @@ class Rotary:
 
 
 def _positions(positions, tokens, device):
-    _need(positions.dtype in (torch.int64, torch.int32) and positions.is_contiguous() and positions.numel() == tokens,
-          "positions: %d contiguous int64 or int32 values are wanted" % tokens)
-    _need(positions.device == device, "positions are on %s, the tensors on %s" % (positions.device, device))
-    return positions.data_ptr(), positions.element_size()
+    size = 8 if positions.dtype == torch.int64 else 4 if positions.dtype == torch.int32 else 0
+    if not size or positions.numel() != tokens or not positions.is_contiguous():
+        _refuse("positions: %d contiguous int64 or int32 values are wanted" % tokens)
+    if positions.device != device:
+        _refuse("positions are on %s, the tensors on %s" % (positions.device, device))
+    return positions.data_ptr(), size
 
 
 def rotary(plan, x, positions, out=None, inverse=False):
     """x [tokens, heads, head_dim] with every head turned to its token's position [tokens] (any sign), into `out` (may be x; default: a
     new tensor).  inverse=True turns back: the gradient of rotary() with respect to x, given the gradient of its result."""
-    _need(x.dim() == 3 and x.dtype in _DTYPES, "x is %s %s: [tokens, heads, head_dim] in float32, float16 or bfloat16 is wanted"
-          % (x.dtype, tuple(x.shape)))
-    tokens, heads, dim = x.shape
-    _need(dim == plan.head_dim, "x has heads of %d channels, the plan of %d" % (dim, plan.head_dim))
-    xt, xh = _rows(x, "x", (heads, dim), x.dtype, x.device)
-    pp, pb = _positions(positions, tokens, x.device)
-    _need(plan.device == x.device, "the plan is on %s, x on %s" % (plan.device, x.device))
+    shape, dtype, device = x.shape, x.dtype, plan.device
+    kind = _DTYPES.get(dtype)
+    if kind is None or len(shape) != 3:
+        _refuse("x is %s %s: [tokens, heads, head_dim] in float32, float16 or bfloat16 is wanted" % (dtype, list(shape)))
+    tokens, heads, dim = shape
+    if dim != plan.head_dim:
+        _refuse("x has heads of %d channels, the plan of %d" % (dim, plan.head_dim))
+    xt, xh = _rows(x, "x", shape, dtype, device)
+    pp, pb = _positions(positions, tokens, device)
     _lib.require_gpu(x, "x")
-    y = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device) if out is None else out
-    yt, yh = _rows(y, "out", (heads, dim), x.dtype, x.device)
-    _need(y.shape[0] == tokens, "out has %d tokens, x %d" % (y.shape[0], tokens))
-    a = _RotaryArgs(x.data_ptr(), y.data_ptr(), xt, xh, yt, yh, pp, pb, tokens, heads, dim, _DTYPES[x.dtype], int(inverse))
-    _queue("rotary", x.device, ctypes.byref(a), ctypes.c_void_p(plan._ref))
+    if out is None:
+        y, yt, yh = torch.empty(shape, dtype=dtype, device=device), heads * dim, dim
+    else:
+        y, (yt, yh) = out, _rows(out, "out", shape, dtype, device)
+    _queue("rotary", device, _PACK_ROTARY(x.data_ptr(), y.data_ptr(), xt, xh, yt, yh, pp, pb, tokens, heads, dim, kind, 1 if inverse else 0), plan._ref)
     return y
 
 
@@ -1005,43 +1025,48 @@ class PagedBatch:
                               block_table.shape[1], batch, self.max_new, 0 if max_len is None else int(max_len))
         self._ref = ctypes.addressof(self._c)
 
-    def _for(self, cache):
-        _need(self.device == cache.device, "the batch is on %s, the cache on %s" % (self.device, cache.device))
-        return ctypes.c_void_p(self._ref)
+
+def _same_device(batch, cache):
+    if batch.device != cache.device:
+        _refuse("the batch is on %s, the cache on %s" % (batch.device, cache.device))
 
 
 def kv_append(cache, batch, k, v, rotary=None, q=None, positions=None, q_out=None):
     """Writes k, v [tokens, kv_heads, head_dim] of the batch's new tokens to their places in the cache; with a `rotary` plan the keys, and
     q [tokens, q_heads, head_dim] if given, turn on the way.  Returns the turned q (in `q_out`, which may be q; default: a new tensor), or
     None.  Tokens turn by their place in the cache, or by `positions` [tokens].  One launch."""
-    tokens = k.shape[0]
-    kt, kh = _rows(k, "k", (cache.kv_heads, cache.head_dim), cache.dtype, cache.device)
-    vt, vh = _rows(v, "v", (cache.kv_heads, cache.head_dim), cache.dtype, cache.device)
-    _need(v.shape[0] == tokens, "k has %d tokens, v %d" % (tokens, v.shape[0]))
-    a = _KvAppendArgs(k.data_ptr(), v.data_ptr(), kt, kh, vt, vh)
-    a.tokens = tokens
-    if q is not None:
-        _need(q.dim() == 3 and q.shape[0] == tokens and q.shape[1] > 0, "q is %s: [%d, q_heads, head_dim] is wanted" % (tuple(q.shape), tokens))
-        shape = (q.shape[1], cache.head_dim)
-        a.q_tstride, a.q_hstride = _rows(q, "q", shape, cache.dtype, cache.device)
-    else:
-        _need(q_out is None, "q_out without q")
-    if positions is not None:
-        _need(rotary is not None, "positions without a rotary plan")
-        a.positions, a.position_bytes = _positions(positions, tokens, cache.device)
+    tokens, dtype, device = k.shape[0], cache.dtype, cache.device
+    shape = (tokens, cache.kv_heads, cache.head_dim)
+    kt, kh = _rows(k, "k", shape, dtype, device)
+    vt, vh = _rows(v, "v", shape, dtype, device)
+    pp = pb = plan = None
     if rotary is not None:
-        _need(rotary.head_dim == cache.head_dim and rotary.device == cache.device,
-              "the plan is for heads of %d on %s, the cache has %d on %s" % (rotary.head_dim, rotary.device, cache.head_dim, cache.device))
-    ref = batch._for(cache)
-    _lib.require_gpu(k, "k")
-    if q is not None:
+        plan = rotary._ref
+        if rotary.head_dim != cache.head_dim or rotary.device != device:
+            _refuse("the plan is for heads of %d on %s, the cache has %d on %s" % (rotary.head_dim, rotary.device, cache.head_dim, device))
+        if positions is not None:
+            pp, pb = _positions(positions, tokens, device)
+    elif positions is not None:
+        _refuse("positions without a rotary plan")
+    _same_device(batch, cache)
+    if q is None:
+        if q_out is not None:
+            _refuse("q_out without q")
+        _lib.require_gpu(k, "k")
+        tail = (0, 0, 0, 0, 0, 0, pp or 0, pb or 0, tokens, 0)
+    else:
+        qs = q.shape
+        if len(qs) != 3 or qs[1] == 0:
+            _refuse("q is %s: [%d, q_heads, head_dim] is wanted" % (list(qs), tokens))
+        qs = (tokens, qs[1], cache.head_dim)
+        qt, qh = _rows(q, "q", qs, dtype, device)
+        _lib.require_gpu(k, "k")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_out, ot, oh = torch.empty(qs, dtype=dtype, device=device), qs[1] * qs[2], qs[2]
         else:
-            _need(q_out.shape == q.shape, "q_out is %s, q %s" % (tuple(q_out.shape), tuple(q.shape)))
-        a.qo_tstride, a.qo_hstride = _rows(q_out, "q_out", shape, cache.dtype, cache.device)
-        a.q, a.q_out, a.q_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
-    _queue("kv_append", cache.device, ctypes.byref(a), ctypes.c_void_p(cache._ref), ref, ctypes.c_void_p(rotary._ref) if rotary is not None else None)
+            ot, oh = _rows(q_out, "q_out", qs, dtype, device)
+        tail = (q.data_ptr(), q_out.data_ptr(), qt, qh, ot, oh, pp or 0, pb or 0, tokens, qs[1])
+    _queue("kv_append", device, _PACK_APPEND(k.data_ptr(), v.data_ptr(), kt, kh, vt, vh, *tail), cache._ref, batch._ref, plan)
     return q_out
 
 
@@ -1050,22 +1075,33 @@ def paged_attention(q, cache, batch, scale=None, causal=True, window=0, out=None
     up to itself (causal) and no further back than `window` tokens, itself among them (0: all).  q_heads: a multiple of the cache's heads,
     head h reads key head h // (q_heads // kv_heads).  scale: default head_dim ** -0.5.  A token that sees no key gets zeros; rows of
     `out` behind the last sequence are left as they were."""
-    _need(q.dim() == 3 and q.shape[1] > 0 and q.shape[1] % cache.kv_heads == 0,
-          "q is %s: [tokens, a multiple of %d heads, head_dim] is wanted" % (tuple(q.shape), cache.kv_heads))
-    tokens, heads, dim = q.shape
-    qt, qh = _rows(q, "q", (heads, cache.head_dim), cache.dtype, cache.device)
-    _need(0 <= window < 2 ** 31, "window %d" % window)
-    ref = batch._for(cache)
+    dtype, device, dim = cache.dtype, cache.device, cache.head_dim
+    shape = q.shape
+    if len(shape) != 3 or shape[1] == 0 or shape[1] % cache.kv_heads:
+        _refuse("q is %s: [tokens, a multiple of %d heads, head_dim] is wanted" % (list(shape), cache.kv_heads))
+    shape = (shape[0], shape[1], dim)
+    qt, qh = _rows(q, "q", shape, dtype, device)
+    if not 0 <= window < 2 ** 31:
+        _refuse("window %d" % window)
+    _same_device(batch, cache)
     _lib.require_gpu(q, "q")
-    o = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device) if out is None else out
-    ot, oh = _rows(o, "out", (heads, dim), cache.dtype, cache.device)
-    _need(o.shape[0] == tokens, "out has %d tokens, q %d" % (o.shape[0], tokens))
-    a = _PagedAttentionArgs(q.data_ptr(), o.data_ptr(), 0 if tokens <= 1 else qt, 0 if heads <= 1 else qh, 0 if tokens <= 1 else ot,
-                            0 if heads <= 1 else oh, tokens, heads, int(bool(causal)), int(window), dim ** -0.5 if scale is None else float(scale))
-    need = lib().ttsamd_paged_attention_workspace_bytes(ctypes.byref(a), ctypes.c_void_p(cache._ref), ref)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _queue("paged_attention", cache.device, ctypes.byref(a), ctypes.c_void_p(cache._ref), ref, P(ws), ctypes.c_size_t(need))
+    if out is None:
+        o, ot, oh = torch.empty(shape, dtype=dtype, device=device), shape[1] * dim, dim
+    else:
+        o, (ot, oh) = out, _rows(out, "out", shape, dtype, device)
+    a = _PACK_ATTENTION(q.data_ptr(), o.data_ptr(), qt, qh, ot, oh, shape[0], shape[1], 1 if causal else 0, window, dim ** -0.5 if scale is None else scale)
+    need = _workspace_bytes()(a, cache._ref, batch._ref)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _queue("paged_attention", device, a, cache._ref, batch._ref, ws.data_ptr() if need else None, need)
     return o
+
+
+def _workspace_bytes():
+    fn = _FNS.get("workspace")
+    if fn is None:
+        fn = _FNS["workspace"] = lib().ttsamd_paged_attention_workspace_bytes
+        fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_void_p]
+    return fn
 
 
 class PackedW4:
@@ -1082,7 +1118,7 @@ class PackedW4:
         group = k // scales.shape[1]
         _need(n > 0 and group in (32, 64, 128) and group * scales.shape[1] == k, "groups of %d: 32, 64 or 128, k a multiple of it" % group)
         _need(zeros is None or (zeros.dtype == torch.uint8 and zeros.shape == scales.shape), "zeros: uint8, shaped as the scales")
-        _need(bias is None or tuple(bias.shape) == (n,), "bias: [n]")
+        _need(bias is None or (tuple(bias.shape) == (n,) and bias.is_contiguous() and bias.dtype in _DTYPES), "bias: [n], contiguous")
         _need(all(t is None or t.device == qweight.device for t in (scales, zeros, bias)), "qweight, scales, zeros and bias are on one device")
         tiles, chunks = -(-n // 16), -(-k // 128)
         per = 128 // group
@@ -1103,6 +1139,9 @@ class PackedW4:
         self.zeros = None if zeros is None else by_group(zeros)
         self.bias = bias
         self.n, self.k, self.group, self.device = n, k, group, qweight.device
+        self.bias_dtype = None if bias is None else bias.dtype
+        self._scale_kind = _DTYPES[scales.dtype]
+        self._pointers = tuple(0 if t is None else t.data_ptr() for t in (self.levels, self.scales, self.zeros, bias))
 
     @classmethod
     def quantize(cls, weight, group=64, bias=None, zeros=False, scale_dtype=None):
@@ -1130,17 +1169,23 @@ def linear_w4(weights, x, out=None):
     """x [rows, k] times the packed weights [n, k] transposed, plus their bias -> [rows, n] in x's type (float32, float16, bfloat16).
     Meant for the few rows of a decoding step; any number is computed."""
     w = weights
-    _need(x.dim() == 2 and x.shape[1] == w.k and x.dtype in _DTYPES, "x is %s %s: [rows, %d] in float32, float16 or bfloat16 is wanted"
-          % (x.dtype, tuple(x.shape), w.k))
-    _need(x.stride(1) == 1, "the channels of a row of x have to be contiguous")
-    _need(x.device == w.device and (w.bias is None or w.bias.dtype == x.dtype), "x is %s on %s, the layer %s on %s"
-          % (x.dtype, x.device, x.dtype if w.bias is None else w.bias.dtype, w.device))
+    shape, dtype, device = x.shape, x.dtype, w.device
+    kind = _DTYPES.get(dtype)
+    if kind is None or len(shape) != 2 or shape[1] != w.k:
+        _refuse("x is %s %s: [rows, %d] in float32, float16 or bfloat16 is wanted" % (dtype, list(shape), w.k))
+    xs, xd = x.stride()
+    if xd != 1:
+        _refuse("the channels of a row of x have to be contiguous")
+    if x.device != device or w.bias_dtype not in (None, dtype):
+        _refuse("x is %s on %s, the layer %s on %s" % (dtype, x.device, w.bias_dtype or dtype, device))
     _lib.require_gpu(x, "x")
-    m = x.shape[0]
-    y = torch.empty((m, w.n), dtype=x.dtype, device=x.device) if out is None else out
-    _need(y.shape == (m, w.n) and y.dtype == x.dtype and y.device == x.device and (w.n == 1 or y.stride(1) == 1),
-          "out: [%d, %d] %s with contiguous rows is wanted" % (m, w.n, x.dtype))
-    a = _LinearW4Args(x.data_ptr(), y.data_ptr(), x.stride(0), y.stride(0), w.levels.data_ptr(), w.scales.data_ptr(), _dp(w.zeros), _dp(w.bias),
-                      m, w.n, w.k, w.group, _DTYPES[x.dtype], _DTYPES[w.scales.dtype])
-    _queue("linear_w4", x.device, ctypes.byref(a))
+    m, n = shape[0], w.n
+    if out is None:
+        y, ys = torch.empty((m, n), dtype=dtype, device=device), n
+    else:
+        y = out
+        if y.shape != (m, n) or y.dtype != dtype or y.device != device or (y.stride(1) != 1 and n > 1):
+            _refuse("out: [%d, %d] %s on %s with contiguous rows is wanted" % (m, n, dtype, device))
+        ys = y.stride(0)
+    _queue("linear_w4", device, _PACK_W4(x.data_ptr(), y.data_ptr(), xs, ys, *w._pointers, m, n, w.k, w.group, kind, w._scale_kind))
     return y
