@@ -32,7 +32,7 @@ def places(table, seq_lens, q_starts, page_size, pages, tokens):
 
 
 def attend(q, k_cache, v_cache, table, seq_lens, q_starts, scale, causal=True, window=0):
-    """-> out [tokens, heads, dim] (NaN in rows no sequence owns), the sum of p |v| per value, and the largest sum of |q k| * scale."""
+    """-> out [tokens, heads, dim] (NaN in rows no sequence owns), the sum of p |v| per value, and the largest sum of |q k scale|."""
     tokens, heads, dim = q.shape
     pages, kv_heads, page_size, _ = k_cache.shape
     g = heads // kv_heads
@@ -65,7 +65,7 @@ def attend(q, k_cache, v_cache, table, seq_lens, q_starts, scale, causal=True, w
                 out[start + i, h] = p[i, row] @ vh[row]
                 mag[start + i, h] = p[i, row] @ vh[row].abs()
                 if bool(row.any()):
-                    reach = max(reach, float((qh[i].abs() @ kh[row].abs().T).max()) * scale)
+                    reach = max(reach, float((qh[i].abs() @ kh[row].abs().T).max()) * abs(scale))     # a score is off by its size, whatever its sign
     return out, mag, reach
 
 

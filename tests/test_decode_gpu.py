@@ -210,7 +210,10 @@ ATTEND = [
     ([1], [700], 2, 34, 96, 16), ([1, 1], [300, 50], 1, 1, 256, 128), ([1], [513], 3, 3, 40, 7),
     # chunks
     ([2], [2], 1, 1, 64, 16), ([17, 1, 33], [17, 40, 33], 2, 2, 64, 16), ([5, 64], [100, 64], 1, 3, 128, 1), ([70], [333], 2, 4, 72, 24),
-    ([129, 128, 127], [129, 200, 500], 1, 2, 128, 64), ([40], [40], 1, 8, 256, 16), ([300], [310], 2, 2, 32, 13), ([9, 6], [4, 6], 1, 2, 64, 8)]
+    ([129, 128, 127], [129, 200, 500], 1, 2, 128, 64), ([40], [40], 1, 8, 256, 16), ([300], [310], 2, 2, 32, 13), ([9, 6], [4, 6], 1, 2, 64, 8),
+    # chunks with enough rows to be staged for 128 at a time: whole and part tiles, all widths of a head
+    ([129, 64, 1, 33, 70], [129, 190, 400, 33, 65], 16, 16, 64, 16), ([40, 90], [40, 350], 16, 64, 128, 64), ([33, 34], [97, 40], 16, 64, 80, 1),
+    ([70, 10], [77, 300], 16, 32, 256, 24), ([65, 100], [500, 99], 32, 32, 40, 32), ([128, 128], [256, 129], 16, 32, 200, 8)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
@@ -226,17 +229,18 @@ def test_paged_attention(gpu, dtype, new, lens, kv, heads, dim, page):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("new,lens,window", [([1, 1], [200, 33], 0), ([40, 3], [200, 33], 0), ([40, 90], [200, 90], 50), ([1], [90], 1)])
-def test_paged_attention_not_causal(gpu, dtype, new, lens, window):
-    c = Case(gpu, dtype, new, lens, 2, 4, 64, 16, seed=7)
+@pytest.mark.parametrize("new,lens,window,kv", [([1, 1], [200, 33], 0, 2), ([40, 3], [200, 33], 0, 2), ([40, 90], [200, 90], 50, 2), ([1], [90], 1, 2),
+                                                ([40, 65], [200, 90], 50, 32), ([70], [140], 0, 64)])
+def test_paged_attention_not_causal(gpu, dtype, new, lens, window, kv):
+    c = Case(gpu, dtype, new, lens, kv, 2 * kv, 64, 16, seed=7)
     c.check(ops.paged_attention(c.q.to(gpu), c.cache, c.batch, causal=False, window=window), causal=False, window=window)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("new", [1, 20, 150])
-def test_paged_attention_bad_pages_and_sizes_hold_no_key(gpu, dtype, new):
+@pytest.mark.parametrize("new,kv", [(1, 2), (20, 2), (150, 2), (100, 32)])
+def test_paged_attention_bad_pages_and_sizes_hold_no_key(gpu, dtype, new, kv):
     """Pages outside the pool, a table narrower than the lengths, starts beyond the tokens: what is there is attended, nothing faults."""
-    c = Case(gpu, dtype, [new, new], [160, 170], 2, 4, 64, 16, seed=new)
+    c = Case(gpu, dtype, [new, new], [160, 170], kv, kv if kv > 2 else 4, 64, 16, seed=new)
     for col, page in ((0, -3), (3, 10 ** 6), (9, 2 ** 31 - 1)):
         c.table[0, col] = page
     c.table = c.table[:, :10].contiguous()                            # sequence 1 reaches position 169: its last keys have no column
@@ -253,37 +257,42 @@ def test_paged_attention_bad_pages_and_sizes_hold_no_key(gpu, dtype, new):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-def test_paged_attention_computes_more_than_it_was_sized_for(gpu, dtype):
-    c = Case(gpu, dtype, [70, 1, 200], [90, 400, 250], 2, 4, 64, 16, seed=2)
-    for most in ((1, 1), (0, 0), (7, 40)):
+@pytest.mark.parametrize("kv", [2, 32])
+def test_paged_attention_computes_more_than_it_was_sized_for(gpu, dtype, kv):
+    c = Case(gpu, dtype, [70, 1, 200], [90, 400, 250], kv, kv if kv > 2 else 4, 64, 16, seed=2)
+    for most in ((1, 1), (0, 0), (7, 40), (65, 100)):
         c.batch = ops.PagedBatch(c.table.to(gpu), c.batch.seq_lens, c.batch.q_starts, max_new=most[0], max_len=most[1])
         c.check(ops.paged_attention(c.q.to(gpu), c.cache, c.batch), what=str(most))
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("new", [1, 90])
-def test_paged_attention_strides_and_large_scores(gpu, dtype, new):
-    """A layer's slice of a cache of many layers, q as a slice of one projection, out in a wider tensor; scores in the hundreds."""
-    c = Case(gpu, dtype, [new, new], [300, 120], 2, 4, 64, 16, seed=4)
+@pytest.mark.parametrize("new,kv,scale", [(1, 2, None), (90, 2, None), (70, 32, None), (70, 32, -0.2), (70, 32, 0.0), (1, 2, -0.2), (1, 2, 0.0)])
+def test_paged_attention_strides_and_large_scores(gpu, dtype, new, kv, scale):
+    """A layer's slice of a cache of many layers, q as a slice of one projection, out in a wider tensor; scores in the hundreds; scales that
+    are negative or zero."""
+    heads = kv if kv > 2 else 4
+    c = Case(gpu, dtype, [new, new], [300, 120], kv, heads, 64, 16, seed=4)
     pages = c.k.shape[0]
-    pool = torch.full((pages, 3, 2, 16, 2, 64), math.nan, dtype=dtype, device=gpu)    # [pages, layers, k/v, rows, heads, dim]
+    pool = torch.full((pages, 3, 2, 16, kv, 64), math.nan, dtype=dtype, device=gpu)   # [pages, layers, k/v, rows, heads, dim]
     pool[:, 1, 0], pool[:, 1, 1] = c.k.to(gpu).transpose(1, 2), c.v.to(gpu).transpose(1, 2)
     cache = ops.PagedKV(pool[:, 1, 0].transpose(1, 2), pool[:, 1, 1].transpose(1, 2))
-    fused = torch.randn(c.tokens, 8, 64, generator=_g(1)).to(dtype).to(gpu)
-    fused[:, 2:6] = (c.q * 20).to(gpu)
-    wide = torch.full((c.tokens, 6, 64), 3.0, dtype=dtype, device=gpu)
-    ops.paged_attention(fused[:, 2:6], cache, c.batch, out=wide[:, 1:5])
-    assert bool((wide[:, 0] == 3).all()) and bool((wide[:, 5] == 3).all())
-    c.q = fused[:, 2:6].cpu()
-    c.check(wide[:, 1:5], what="strided")
+    fused = torch.randn(c.tokens, heads + 4, 64, generator=_g(1)).to(dtype).to(gpu)
+    mine = fused[:, 2: heads + 2]
+    mine.copy_((c.q * 20).to(gpu))
+    wide = torch.full((c.tokens, heads + 2, 64), 3.0, dtype=dtype, device=gpu)
+    ops.paged_attention(mine, cache, c.batch, scale=scale, out=wide[:, 1: heads + 1])
+    assert bool((wide[:, 0] == 3).all()) and bool((wide[:, heads + 1] == 3).all())
+    c.q = mine.cpu()
+    c.check(wide[:, 1: heads + 1], scale=scale, what="strided")
 
 
+@pytest.mark.parametrize("kv", [1, 32])
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-def test_paged_attention_non_finite_values_reach_only_who_sees_them(gpu, dtype):
+def test_paged_attention_non_finite_values_reach_only_who_sees_them(gpu, dtype, kv):
     """NaN and infinities in keys or values of tokens that a row does not see (later ones of its chunk, those out of its window) take no
     part in it."""
     new, n = 100, 180
-    c = Case(gpu, dtype, [new], [n], 1, 2, 64, 16, seed=8)
+    c = Case(gpu, dtype, [new], [n], kv, 2 * kv, 64, 16, seed=8)
     for j, value in ((120, math.nan), (150, math.inf), (171, -math.inf)):
         page, row = int(c.table[0, j // 16]), j % 16
         (c.cache.k if j == 150 else c.cache.v)[page, :, row, 5] = value

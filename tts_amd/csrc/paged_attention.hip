@@ -2,7 +2,7 @@
 //
 // out[t,h] = sum_j p_j v_j, p = softmax_j(scale q.k_j) over the keys token t sees, in one pass over the keys with a running maximum m
 // and sum l: a tile's scores s give m' = max(m, s), p = exp(s - m'), l = l exp(m - m') + sum p, o = o exp(m - m') + sum p v.
-#include "paged_stream.h"
+#include "paged_tile.h"
 
 namespace ttsamd {
 namespace {
@@ -10,6 +10,7 @@ namespace {
 constexpr int kCus = 256;
 
 struct Launch {
+    bool tile;                       // paged_tile.h; else paged_stream.h
     int dp, nq, waves, splits, split_keys, row_tiles;
     size_t part_bytes, stat_bytes;
 };
@@ -25,6 +26,12 @@ Launch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv &c, c
     const int group = a.q_heads / c.kv_heads;
     p.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
     const int64_t rows = (int64_t)(b.max_new < 1 ? 1 : b.max_new) * group;
+    const int64_t tile_blocks = (rows + kTileRows - 1) / kTileRows * c.kv_heads * b.batch;
+    if (!f32 && rows >= 64 && tile_blocks >= 64) {
+        p.tile = true, p.splits = 1;
+        p.row_tiles = (int)((rows + kTileRows - 1) / kTileRows < 65535 ? (rows + kTileRows - 1) / kTileRows : 65535);
+        return p;
+    }
     p.nq = rows > 16 && p.dp < 256 ? 2 : 1;
     const int64_t tiles = (rows + 16 * p.nq - 1) / (16 * p.nq);
     p.row_tiles = (int)(tiles < 65535 ? tiles : 65535);
@@ -63,8 +70,24 @@ template <class T, int DP, int NQ> hipError_t start(const AttArgs &g, const Laun
 {
     return g.c.head_dim == DP ? start<T, DP, NQ, true>(g, p, grid, st) : start<T, DP, NQ, false>(g, p, grid, st);
 }
+template <class T, int DP, bool FULL> hipError_t start_tile(const AttArgs &g, dim3 grid, hipStream_t st)
+{
+    static std::atomic<unsigned long long> done{0};
+    constexpr int bytes = 2 * 2 * kTileKeys * DP * 2;
+    if (hipError_t e = ensure_dynamic_lds((const void *)attend_tile<T, DP, FULL>, bytes, done)) return e;
+    attend_tile<T, DP, FULL><<<grid, 256, bytes, st>>>(g);
+    return hipSuccess;
+}
+template <class T, int DP> hipError_t start_tile(const AttArgs &g, dim3 grid, hipStream_t st)
+{
+    return g.c.head_dim == DP ? start_tile<T, DP, true>(g, grid, st) : start_tile<T, DP, false>(g, grid, st);
+}
 template <class T> hipError_t start(const AttArgs &g, const Launch &p, hipStream_t st)
 {
+    if constexpr (sizeof(T) == 2) {
+        const dim3 grid(g.c.kv_heads, p.row_tiles, g.b.batch);
+        if (p.tile) return p.dp == 64 ? start_tile<T, 64>(g, grid, st) : p.dp == 128 ? start_tile<T, 128>(g, grid, st) : start_tile<T, 256>(g, grid, st);
+    }
     const dim3 grid(g.c.kv_heads * p.splits, p.row_tiles, g.b.batch);
     if (p.dp == 64) return p.nq == 2 ? start<T, 64, 2>(g, p, grid, st) : start<T, 64, 1>(g, p, grid, st);
     if (p.dp == 128) return p.nq == 2 ? start<T, 128, 2>(g, p, grid, st) : start<T, 128, 1>(g, p, grid, st);

@@ -77,9 +77,9 @@ template <class T> __device__ __forceinline__ bool any_odd(unsigned w)
 }
 
 // One row's keys [lo, hi), a wave, key by key: o[d] += p v only for the keys of `see`.  For the rare tile where a value that some row
-// must not see is an infinity or NaN.
+// must not see is an infinity or NaN.  Lane x owns o[x], o[x + 64], ..; returns the sum of the p (every lane).
 template <class T>
-__device__ void attend_row(const AttArgs &g, int b, int hk, const T *q, Range see, float *o, float *ml)
+__device__ float attend_row(const AttArgs &g, int b, int hk, const T *q, Range see, float *o, float *ml)
 {
     const int lane = threadIdx.x & 63, D = g.c.head_dim;
     float m = kNoMax, l = 0.f, acc[4] = {};
@@ -100,6 +100,7 @@ __device__ void attend_row(const AttArgs &g, int b, int hk, const T *q, Range se
     for (int y = 0; y < 4; ++y)
         if (lane + 64 * y < D) o[lane + 64 * y] = acc[y];
     if (lane == 0) ml[0] = m, ml[1] = l;
+    return l;
 }
 
 template <class T, int DP, int NQ, bool FULL, int MAXW>

@@ -1,0 +1,244 @@
+// Attention of many rows over a paged cache (chunks of a prompt), 16-bit types: keys and values staged through LDS for 128 rows.
+//
+// A workgroup takes 128 rows (row = token x heads of one key head, as in paged_stream.h), 32 a wave, and walks the keys 64 at a time.
+// As there, S^T = K Q^T is computed, here in 32x32x16 products: a lane holds one row (column lane % 32) and half of a tile's keys, the
+// probabilities are the right operand of O^T = V^T P^T where they lie (slot e of half h of product u is key 16 u + 4 h + e, + 4 for
+// e >= 4), and V^T comes out of LDS by the transposing read, four keys of a channel at a time.
+//
+// LDS.  Two buffers of 64 key rows and 64 value rows: while a tile is multiplied the next one's keys, then its values, travel through
+// registers into the other buffer; one barrier a tile.  A row's 16-byte pieces are permuted by an exclusive or with a function of the row,
+// so that the reads of 8 (and 16) neighbouring lanes fall on different banks: keys are read a piece a row down a column, values 32 (64)
+// bytes of four rows.
+//
+// Bound: the matrix unit, with the exponentials (a quarter of the vector rate) next to it.
+#pragma once
+#include "paged_stream.h"
+
+namespace ttsamd {
+
+template <class T> __device__ __forceinline__ f32x16_t mfma_32x32x16(uint4 a, uint4 b, f32x16_t c)
+{
+    if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// Both halves of w, added to c in fp32.
+template <class T> __device__ __forceinline__ float sum2(unsigned w, float c)
+{
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), b2{(__bf16)1.f, (__bf16)1.f}, c, false);
+    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), h2{(_Float16)1.f, (_Float16)1.f}, c, false);
+}
+
+constexpr int kTileRows = 128, kTileKeys = 64;
+
+template <class T, int DP, bool FULL>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
+{
+    constexpr int CH = DP / 8, RB = DP * 2, NSTG = CH / 4, RPI = 64 / CH, NS = DP / 16, ND = DP / 32;
+    constexpr int HALF = kTileKeys * RB;                    // bytes of a tile's keys (or values)
+    extern __shared__ float lds_f[];
+    char *const lds = (char *)lds_f;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c32 = lane & 31, h2 = lane >> 5;
+    const int hk = blockIdx.x, b = blockIdx.z;
+    const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, b);
+    const int D = g.c.head_dim, rows = s.n * g.group, tiles = (rows + kTileRows - 1) / kTileRows;
+    const char *kbase = (const char *)g.c.k + (int64_t)hk * g.c.k_head * 2, *vbase = (const char *)g.c.v + (int64_t)hk * g.c.v_head * 2;
+    const uint32_t kpage16 = (uint32_t)(g.c.k_page / 8), krow16 = (uint32_t)(g.c.k_row / 8);
+    const uint32_t vpage16 = (uint32_t)(g.c.v_page / 8), vrow16 = (uint32_t)(g.c.v_row / 8);
+    auto k_swz = [](int row) { return CH == 8 ? (row & 7) ^ (row >> 3 & 1) : row & 15; };
+    auto v_swz = [](int row) { return CH == 8 ? (row & 3) << 1 : (row & 1) << 2 | (row & 2) * 5; };     // 0 4 10 14
+
+    // staging: this thread's piece of NSTG rows
+    const int piece = lane % CH, row_of_lane = lane / CH;
+    const bool piece_in = FULL || piece * 8 < D;
+    const char *kbase_l = kbase + (piece_in ? piece * 16 : 0), *vbase_l = vbase + (piece_in ? piece * 16 : 0);
+    // reading: a key row per lane; four value rows and a 32-byte span per 16 lanes
+    const int i16 = lane & 15, vr = 4 * h2 + (i16 >> 2), vc = 2 * (lane >> 4 & 1) + (i16 >> 1 & 1), vb8 = (i16 & 1) * 8;
+
+    // the largest score is found before the scale: it has to be positive (a negative one turns q's sign, zero takes q away)
+    const unsigned flip = g.scale2 < 0.f ? 0x80008000u : 0u, keep = g.scale2 == 0.f ? 0u : ~0u;
+    const float scale2 = g.scale2 == 0.f ? 1.f : fabsf(g.scale2);
+    for (int tile = tiles - 1 - blockIdx.y; tile >= 0; tile -= gridDim.y) {         // the longest first
+        const int r0 = tile * kTileRows, last = min(r0 + kTileRows, rows) - 1, w0 = min(r0 + 32 * wave, last), w1 = min(r0 + 32 * wave + 31, last);
+        auto range_of = [&](int r) { return seen_by(s, s.len - s.n + (int)g.by_group.div(r), g.a.causal, g.a.window); };
+        const int my_row = min(r0 + 32 * wave + c32, last), my_i = g.by_group.div(my_row), my_h = hk * g.group + my_row - my_i * g.group;
+        const Range mine = range_of(my_row), wfirst = range_of(w0), wlast = range_of(w1), first = range_of(r0), final = range_of(last);
+        uint4 q[NS];
+        {
+            const char *src = (const char *)g.a.q + ((int64_t)(s.start + my_i) * g.a.q_tstride + (int64_t)my_h * g.a.q_hstride) * 2;
+#pragma unroll
+            for (int x = 0; x < NS; ++x) {
+                const bool in = FULL || x * 16 + h2 * 8 < D;
+                q[x] = in ? *(const uint4 *)(src + (in ? x * 32 + h2 * 16 : 0)) : uint4{0, 0, 0, 0};
+                q[x].x = (q[x].x & keep) ^ flip, q[x].y = (q[x].y & keep) ^ flip, q[x].z = (q[x].z & keep) ^ flip, q[x].w = (q[x].w & keep) ^ flip;
+            }
+        }
+        f32x16_t o[ND];
+#pragma unroll
+        for (int x = 0; x < ND; ++x)
+#pragma unroll
+            for (int y = 0; y < 16; ++y) o[x][y] = 0.f;
+        float m = kNoMax, l = 0.f;
+        bool odd = false;
+
+        const int lo = first.begin, hi = final.end;
+        uint4 st[NSTG];                                      // what travels: keys first, then values
+        auto fetch = [&](int at, int &row) {
+            const int j = at + lane;
+            row = 0;
+            return j < hi ? page_of(g.b, g.by_page, g.c.pages, b, j, row) : -1;
+        };
+        auto stage = [&](const char *src, uint32_t off) {
+#pragma unroll
+            for (int x = 0; x < NSTG; ++x) st[x] = *(const uint4 *)(src + (uint64_t)(uint32_t)__shfl((int)off, (x * 4 + wave) * RPI + row_of_lane) * 16);
+        };
+        auto k_off = [&](int page, int row) { return page < 0 ? 0 : (uint32_t)page * kpage16 + (uint32_t)row * krow16; };
+        auto v_off = [&](int page, int row) { return page < 0 ? 0 : (uint32_t)page * vpage16 + (uint32_t)row * vrow16; };
+        auto put_k = [&](char *buf) {
+#pragma unroll
+            for (int x = 0; x < NSTG; ++x) {
+                const int r = (x * 4 + wave) * RPI + row_of_lane;
+                if (!FULL && !piece_in) st[x] = uint4{0, 0, 0, 0};
+                *(uint4 *)(buf + r * RB + ((piece ^ k_swz(r)) & (CH - 1)) * 16) = st[x];
+            }
+        };
+        auto put_v = [&](char *buf, uint64_t ok, bool mixed) {
+            if (mixed) {
+#pragma unroll
+                for (int x = 0; x < NSTG; ++x) {
+                    if (!(ok >> ((x * 4 + wave) * RPI + row_of_lane) & 1)) st[x] = uint4{0, 0, 0, 0};
+                    odd |= any_odd<T>(st[x].x) || any_odd<T>(st[x].y) || any_odd<T>(st[x].z) || any_odd<T>(st[x].w);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < NSTG; ++x) {
+                const int r = (x * 4 + wave) * RPI + row_of_lane;
+                if (!FULL && !piece_in) st[x] = uint4{0, 0, 0, 0};
+                *(uint4 *)(buf + HALF + r * RB + ((piece ^ v_swz(r)) & (CH - 1)) * 16) = st[x];
+            }
+        };
+        auto mixed_at = [&](int at, uint64_t ok) { return ok != ~0ull || at < final.begin || at + kTileKeys > first.end; };
+
+        int cur = 0, page_next = -1, row_next = 0;
+        uint64_t ok = 0;
+        __syncthreads();                                     // the last row tile's readers are done
+        if (lo < hi) {
+            int row;
+            const int page = fetch(lo, row);
+            ok = __ballot(page >= 0);
+            page_next = fetch(lo + kTileKeys, row_next);
+            stage(kbase_l, k_off(page, row));
+            put_k(lds);
+            stage(vbase_l, v_off(page, row));
+            put_v(lds, ok, mixed_at(lo, ok));
+        }
+        for (int base = lo; base < hi; base += kTileKeys) {
+            __syncthreads();
+            const char *kb = lds + cur * 2 * HALF, *vb = kb + HALF;
+            char *const next = lds + (cur ^ 1) * 2 * HALF;
+            const uint64_t ok_now = ok;
+            const bool more = base + kTileKeys < hi, busy = base < wlast.end && base + kTileKeys > wfirst.begin;
+            uint32_t voff = 0;
+            if (more) {
+                ok = __ballot(page_next >= 0);
+                stage(kbase_l, k_off(page_next, row_next));
+                voff = v_off(page_next, row_next);
+                page_next = fetch(base + 2 * kTileKeys, row_next);
+            }
+            f32x16_t sc[2];
+            if (busy) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    f32x16_t acc;
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) acc[y] = 0.f;
+                    const int r = 32 * t + c32;
+                    const char *kr = kb + r * RB;
+#pragma unroll
+                    for (int x = 0; x < NS; ++x)
+                        acc = mfma_32x32x16<T>(*(const uint4 *)(kr + (((2 * x + h2) ^ k_swz(r)) & (CH - 1)) * 16), q[x], acc);
+                    sc[t] = acc;
+                }
+            }
+            if (more) {
+                put_k(next);
+                stage(vbase_l, voff);
+            }
+            if (busy) {
+                // slot y of half h2 of tile t: key 32 t + 8 (y / 4) + 4 h2 + y % 4
+                if (ok_now != ~0ull || base < wlast.begin || base + kTileKeys > wfirst.end) {
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) {
+                        const int kk = 32 * (y >> 4) + 8 * (y >> 2 & 3) + 4 * h2 + (y & 3), j = base + kk;
+                        if (!(ok_now >> kk & 1) || j < mine.begin || j >= mine.end) sc[y >> 4][y & 15] = -INFINITY;
+                    }
+                }
+                float top = sc[0][0];
+#pragma unroll
+                for (int y = 1; y < 32; ++y) top = fmaxf(top, sc[y >> 4][y & 15]);
+                top *= scale2;
+                if (__any(top > m + kLazy)) {
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const float to = fmaxf(m, top), fade = __builtin_amdgcn_exp2f(m - to);
+                    m = to, l *= fade;
+#pragma unroll
+                    for (int x = 0; x < ND; ++x) o[x] *= fade;
+                }
+#pragma unroll
+                for (int y = 0; y < 32; ++y) sc[y >> 4][y & 15] = __builtin_amdgcn_exp2f(fmaf(sc[y >> 4][y & 15], scale2, -m));
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const f32x16_t &p = sc[u >> 1];
+                    const int y = (u & 1) * 8;
+                    const uint4 pb = {pack2<T>(p[y], p[y + 1]), pack2<T>(p[y + 2], p[y + 3]), pack2<T>(p[y + 4], p[y + 5]), pack2<T>(p[y + 6], p[y + 7])};
+                    l = sum2<T>(pb.x, sum2<T>(pb.y, sum2<T>(pb.z, sum2<T>(pb.w, l))));
+#pragma unroll
+                    for (int x = 0; x < ND; ++x) {
+                        typedef short s4 __attribute__((ext_vector_type(4)));
+                        uint2 part[2];
+#pragma unroll
+                        for (int z = 0; z < 2; ++z) {
+                            const int r = 16 * u + 8 * z + vr;
+                            const char *at = vb + r * RB + (((4 * x + vc) ^ v_swz(r)) & (CH - 1)) * 16 + vb8;
+                            part[z] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)at));
+                        }
+                        o[x] = mfma_32x32x16<T>(uint4{part[0].x, part[0].y, part[1].x, part[1].y}, pb, o[x]);
+                    }
+                }
+            }
+            if (more) put_v(next, ok, mixed_at(base + kTileKeys, ok));
+            cur ^= 1;
+        }
+        const bool redo = __syncthreads_or(odd);
+        if (!redo) {
+            l += __shfl_xor(l, 32);
+            const float inv = l > 0.f ? 1.f / l : l;          // no key: zeros; NaN stays
+            if (r0 + 32 * wave + c32 <= last) {
+                T *dst = (T *)g.a.out + (int64_t)(s.start + my_i) * g.a.o_tstride + (int64_t)my_h * g.a.o_hstride;
+#pragma unroll
+                for (int x = 0; x < ND; ++x)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const int d = 32 * x + 8 * y + 4 * h2;
+                        if (FULL || d < D)
+                            *(uint2 *)(dst + d) = uint2{pack2<T>(o[x][4 * y] * inv, o[x][4 * y + 1] * inv), pack2<T>(o[x][4 * y + 2] * inv, o[x][4 * y + 3] * inv)};
+                    }
+            }
+        } else {
+            float *const mine_o = lds_f + wave * 264;
+            for (int r = r0 + wave; r <= last; r += 4) {
+                const int i = g.by_group.div(r), h = hk * g.group + r - i * g.group;
+                const int64_t token = s.start + i;
+                const float sum = attend_row<T>(g, b, hk, (const T *)g.a.q + token * g.a.q_tstride + (int64_t)h * g.a.q_hstride, range_of(r), mine_o,
+                                                mine_o + 256);
+                const float inv = sum > 0.f ? 1.f / sum : sum;
+                T *dst = (T *)g.a.out + token * g.a.o_tstride + (int64_t)h * g.a.o_hstride;
+                for (int d = lane; d < D; d += 64) dst[d] = (T)(mine_o[d] * inv);
+            }
+        }
+    }
+}
+
+}  // namespace ttsamd
