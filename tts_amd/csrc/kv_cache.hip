@@ -122,11 +122,11 @@ template <class T, int V> __global__ __launch_bounds__(256) void move_rows(MoveA
             } else {
                 dst += (int64_t)token * st.d_t;
             }
-            const int h1 = min(st.heads, (hg + 1) * a.heads_per_unit);
+            const int hstep = (st.heads + a.heads_per_unit - 1) / a.heads_per_unit;     // neighbouring threads take neighbouring heads
             if (chunk >= turning) {
                 const int at = (2 * turning + chunk - turning) * V;
                 if (src + at == dst + at && st.s_h == st.d_h) continue;
-                for (int h = hg * a.heads_per_unit; h < h1; ++h)
+                for (int h = hg; h < st.heads; h += hstep)
                     *(P *)(dst + h * st.d_h + at) = *(const P *)(src + h * st.s_h + at);
                 continue;
             }
@@ -141,7 +141,7 @@ template <class T, int V> __global__ __launch_bounds__(256) void move_rows(MoveA
                 unit_circle(p * a.plan.turns[chunk * V + e], c[e], s[e]);
                 c[e] *= a.plan.amplitude, s[e] *= a.plan.amplitude;
             }
-            for (int h = hg * a.heads_per_unit; h < h1; ++h) {
+            for (int h = hg; h < st.heads; h += hstep) {
                 const P x = *(const P *)(src + h * st.s_h + p0), y = *(const P *)(src + h * st.s_h + p1);
                 P ox, oy;
                 if (a.plan.interleaved) {

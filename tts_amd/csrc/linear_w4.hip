@@ -1,17 +1,17 @@
 // Products of a few rows with 4-bit weights: y[m,n] = sum_g s[n,g] sum_{k in g} x[m,k] (level[n,k] - z[n,g]) + bias[n].
 //
 // Mathematics.  A level q becomes a 16-bit float without arithmetic: its four bits put into the top of the mantissa of 16.0 give 16 + q,
-// exact in bf16 and fp16 alike, two levels for one rotate and one and-or (the image keeps the levels of a word in the order in which
-// the pairs come out).  The matrix unit sums x (16 + q) over a group in fp32, started at -(16 + z) sum x, and the group's scale
-// multiplies what it leaves: no product is rounded before the sum, and what cancels is at most some six times the result's own size.
-// The sums of x come from the matrix unit too (a right operand of ones leaves them in every column, where the start needs them).
+// exact in bf16 and fp16 alike, two levels for one shift and one and-or (the image keeps the levels of a word in the order in which the
+// pairs come out).  The matrix unit sums x (16 + q) over a group in fp32, and x -(16 + z) beside it (a right operand of one value), and
+// the group's scale multiplies what that leaves: no product is rounded before the sum, and what cancels is at most some six times the
+// result's own size.
 // fp32 rows travel as three bf16 parts cut off one after the other (8 + 8 + 8 bits: exact), three products each.
 //
 // Layout.  16x16x32 products with x as the left operand and 16 outputs as the right one: a lane holds the word of 8 levels of output
 // lane % 16, and 16 bytes of the image are the lane's words of four products (128 k): whole lines, read once, straight into registers.
 // x needs no staging either: the lane's eight k are neighbours in memory.  Row r of the left operand is row 4 (r % 4) + r / 4 of x, so
 // that up to four rows land in one accumulator register of every lane.
-// A workgroup owns 16 NT outputs; its waves take the chunks of 128 k in turn and are joined in LDS.
+// A workgroup owns 16 outputs; its waves take the chunks of 128 k in turn and are joined in LDS.
 //
 // Bound: HBM by its bytes (0.5 + scale / group a weight) once the layer is large, the latency of one workgroup for small layers.
 #include "decode_common.h"
@@ -23,167 +23,187 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ unsigned rotr(unsigned x, int n) { return __builtin_amdgcn_alignbit(x, x, n); }
-
-// The eight levels of a word as 16 + q: bits 4p and 16 + 4p of the word hold levels 2p and 2p + 1.
-template <bool BF> __device__ __forceinline__ uint4 unpack(unsigned w)
+// The eight levels of a word as 16 + q: bits 4p and 16 + 4p of the word hold levels 2p and 2p + 1.  `one` is 16.0 twice, in a vector
+// register (and-or takes one scalar operand, the mask).
+template <bool BF> __device__ __forceinline__ uint4 unpack(unsigned w, unsigned one)
 {
     constexpr int at = BF ? 3 : 6;                                     // where the mantissa of 16 + q holds q
-    constexpr unsigned mask = 0xfu << at | 0xfu << (at + 16), one = BF ? 0x41804180u : 0x4c004c00u;
-    return uint4{(rotr(w, (32 - at) & 31) & mask) | one, (rotr(w, (36 - at) & 31) & mask) | one, (rotr(w, (40 - at) & 31) & mask) | one,
-                 (rotr(w, (44 - at) & 31) & mask) | one};
+    constexpr unsigned mask = 0xfu << at | 0xfu << (at + 16);
+    auto field = [&](int bit) { return ((bit < at ? w << (at - bit) : w >> (bit - at)) & mask) | one; };
+    return uint4{field(0), field(4), field(8), field(12)};
 }
 template <bool BF> __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c)
 {
     if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ float ld_any(const void *p, int64_t i, int dtype)
-{
-    return dtype == TTSAMD_F32 ? ((const float *)p)[i] : dtype == TTSAMD_F16 ? to_f(((const _Float16 *)p)[i]) : to_f(((const __bf16 *)p)[i]);
-}
 // The upper halves of x and y.
 __device__ __forceinline__ unsigned uppers(unsigned x, unsigned y) { return __builtin_amdgcn_perm(y, x, 0x07060302u); }
 
-template <class T, int MT, int NT, int GROUP, int MAXW> __global__ __launch_bounds__(MAXW * 64) void linear_w4(ttsamd_linear_w4_args a)
+template <class T, int NT, int GROUP, int MAXW> __global__ __launch_bounds__(MAXW * 64) void linear_w4(ttsamd_linear_w4_args a)
 {
     constexpr bool F32 = sizeof(T) == 4, BF = !__is_same(T, _Float16);
     constexpr int PARTS = F32 ? 3 : 1, PER = GROUP / 32, GPC = 128 / GROUP;      // products a group, groups a chunk
+    constexpr int RAW = F32 ? 2 : 1;                                             // 16-byte pieces of eight k of x
+    constexpr bool XAHEAD = !F32 && NT < 4;
     extern __shared__ float join[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int tiles = (a.n + 15) / 16, chunks = (a.k + 127) / 128;
-    const int n0 = blockIdx.x * NT, m0 = blockIdx.y * 16 * MT, rows = min(a.m - m0, 16 * MT);
+    const int chunks = (a.k + 127) / 128, m0 = blockIdx.y * 16, rows = min(a.m - m0, 16);
     const int c16 = lane & 15, g4 = lane >> 4, row = 4 * (c16 & 3) + (c16 >> 2);
-    const uint4 ones = BF ? uint4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u} : uint4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+    unsigned one = BF ? 0x41804180u : 0x4c004c00u;
+    asm("" : "+v"(one));
     const uint4 *levels[NT];
     int64_t sg[NT];
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-        const int64_t tile = min(n0 + u, tiles - 1);                             // a tile behind the last is computed twice, stored once
+        const int64_t tile = min((int)blockIdx.x * NT + u, (a.n + 15) / 16 - 1);      // behind the last: the last again, never stored
         levels[u] = (const uint4 *)a.levels + tile * chunks * 64 + lane;
         sg[u] = tile * chunks * GPC * 16 + c16;
     }
-    f32x4 acc[NT][MT];
+    // a row behind the last is the last one again: no row of a product meets another
+    const T *const xrow = (const T *)a.x + (int64_t)(m0 + min(row, rows - 1)) * a.x_stride;
+    f32x4 acc[NT];
 #pragma unroll
-    for (int u = 0; u < NT; ++u)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) acc[u][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < NT; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    uint4 next[NT];
-    if (wave < chunks)
-#pragma unroll
-        for (int u = 0; u < NT; ++u) next[u] = levels[u][(int64_t)wave * 64];
-    for (int c = wave; c < chunks; c += waves) {
-        unsigned word[NT][4];
+    // Two chunks are on their way at any time: levels, scales and zeros as they lie in memory, x too where the registers allow.
+    struct Chunk {
+        uint4 word[NT];
+        unsigned scale[NT][GPC], zero[NT][GPC];
+        uint4 x[XAHEAD ? 4 : 1][RAW];
+    } ahead[2];
+    const bool wide = a.scale_dtype == TTSAMD_F32, brain = a.scale_dtype == TTSAMD_BF16, zeros = a.zeros != nullptr;
+    auto fetch_x = [&](uint4(&to)[RAW], int c, int j) {
+        const int k = 128 * c + 32 * j + 8 * g4;                                 // behind the last k the weights are 0: any x will do
+        __builtin_memcpy(to, xrow + (128 * c + 128 <= a.k ? k : min(k, a.k - 8)), 16 * RAW);
+    };
+    auto fetch = [&](Chunk &f, int c) {
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-            word[u][0] = next[u].x, word[u][1] = next[u].y, word[u][2] = next[u].z, word[u][3] = next[u].w;
-            if (c + waves < chunks) next[u] = levels[u][(int64_t)(c + waves) * 64];
+            f.word[u] = levels[u][(int64_t)c * 64];
+#pragma unroll
+            for (int q = 0; q < GPC; ++q) {
+                const int64_t at = sg[u] + ((int64_t)c * GPC + q) * 16;
+                f.scale[u][q] = wide ? ((const unsigned *)a.scales)[at] : ((const unsigned short *)a.scales)[at];
+                if (zeros) f.zero[u][q] = a.zeros[at];
+            }
         }
-        float scale[NT][GPC], zero[NT][GPC];
+        if constexpr (XAHEAD)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) fetch_x(f.x[j], c, j);
+    };
+    auto multiply = [&](Chunk &f, int c) {
+        unsigned word[NT][4], zero[NT][GPC];
+        float scale[NT][GPC];
+        uint4 raw[4][RAW];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            word[u][0] = f.word[u].x, word[u][1] = f.word[u].y, word[u][2] = f.word[u].z, word[u][3] = f.word[u].w;
+#pragma unroll
+            for (int q = 0; q < GPC; ++q) {
+                const unsigned r = f.scale[u][q];
+                scale[u][q] = wide ? __uint_as_float(r) : brain ? __uint_as_float(r << 16) : (float)__builtin_bit_cast(_Float16, (unsigned short)r);
+                // -(16 + z), exact, in both halves
+                const float z = zeros ? -16.f - (float)f.zero[u][q] : -24.f;
+                if constexpr (BF) zero[u][q] = uppers(__float_as_uint(z), __float_as_uint(z));
+                else zero[u][q] = (unsigned)__builtin_bit_cast(unsigned short, (_Float16)z) * 0x10001u;
+            }
+        }
+        if constexpr (XAHEAD)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int y = 0; y < RAW; ++y) raw[j][y] = f.x[j][y];
+        if (c + 2 * waves < chunks) fetch(f, c + 2 * waves);
+        if constexpr (!XAHEAD)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) fetch_x(raw[j], c, j);
+        uint4 x[4][PARTS];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (F32) {
+                unsigned e8[8] = {raw[j][0].x, raw[j][0].y, raw[j][0].z, raw[j][0].w, raw[j][1].x, raw[j][1].y, raw[j][1].z, raw[j][1].w};
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    x[j][p] = uint4{uppers(e8[0], e8[1]), uppers(e8[2], e8[3]), uppers(e8[4], e8[5]), uppers(e8[6], e8[7])};
+                    if (p + 1 < PARTS)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) e8[e] = __float_as_uint(__uint_as_float(e8[e]) - __uint_as_float(e8[e] & 0xffff0000u));
+                }
+            } else {
+                x[j][0] = raw[j][0];
+            }
+        }
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
             for (int q = 0; q < GPC; ++q) {
-                const int64_t at = sg[u] + ((int64_t)c * GPC + q) * 16;
-                scale[u][q] = ld_any(a.scales, at, a.scale_dtype);
-                zero[u][q] = a.zeros ? -16.f - (float)a.zeros[at] : -24.f;
-            }
+                f32x4 part = {0.f, 0.f, 0.f, 0.f};
+                const uint4 start = {zero[u][q], zero[u][q], zero[u][q], zero[u][q]};
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            uint4 x[4][PARTS];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int k = 128 * c + 32 * j + 8 * g4;
-                const bool in = 16 * t + row < rows && k < a.k;
-                const T *src = (const T *)a.x + (int64_t)(m0 + 16 * t + row) * a.x_stride + k;
-                if constexpr (F32) {
-                    unsigned f[8] = {};
-                    if (in) __builtin_memcpy(f, src, 32);
+                for (int j = 0; j < PER; ++j) {
+                    const uint4 w = unpack<BF>(word[u][q * PER + j], one);
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p) {
-                        x[j][p] = uint4{uppers(f[0], f[1]), uppers(f[2], f[3]), uppers(f[4], f[5]), uppers(f[6], f[7])};
-                        if (p + 1 < PARTS)
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) f[e] = __float_as_uint(__uint_as_float(f[e]) - __uint_as_float(f[e] & 0xffff0000u));
+                        part = mfma<BF>(x[q * PER + j][p], start, part);
+                        part = mfma<BF>(x[q * PER + j][p], w, part);
                     }
-                } else {
-                    x[j][0] = uint4{0, 0, 0, 0};
-                    if (in) __builtin_memcpy(&x[j][0], src, 16);
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[u][i] = fmaf(part[i], scale[u][q], acc[u][i]);
             }
-#pragma unroll
-            for (int q = 0; q < GPC; ++q) {
-                f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = 0; j < PER; ++j)
-#pragma unroll
-                    for (int p = 0; p < PARTS; ++p) sum = mfma<BF>(x[q * PER + j][p], ones, sum);
-#pragma unroll
-                for (int u = 0; u < NT; ++u) {
-                    f32x4 part;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) part[i] = sum[i] * zero[u][q];
-#pragma unroll
-                    for (int j = 0; j < PER; ++j) {
-                        const uint4 w = unpack<BF>(word[u][q * PER + j]);
-#pragma unroll
-                        for (int p = 0; p < PARTS; ++p) part = mfma<BF>(x[q * PER + j][p], w, part);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[u][t][i] = fmaf(part[i], scale[u][q], acc[u][t][i]);
-                }
-            }
-        }
+    };
+    if (wave < chunks) fetch(ahead[0], wave);
+    if (wave + waves < chunks) fetch(ahead[1], wave + waves);
+    for (int c = wave; c < chunks; c += 2 * waves) {
+        multiply(ahead[0], c);
+        if (c + waves < chunks) multiply(ahead[1], c + waves);
     }
     // join the waves: [wave][x row][output]
     constexpr int LD = 16 * NT + 1;
 #pragma unroll
     for (int u = 0; u < NT; ++u)
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (16 * t + 4 * i + g4 < rows) join[(wave * rows + 16 * t + 4 * i + g4) * LD + 16 * u + c16] = acc[u][t][i];
+        for (int i = 0; i < 4; ++i)
+            if (4 * i + g4 < rows) join[(wave * rows + 4 * i + g4) * LD + 16 * u + c16] = acc[u][i];
     __syncthreads();
     for (int it = threadIdx.x; it < rows * 16 * NT; it += blockDim.x) {
-        const int r = it / (16 * NT), col = it % (16 * NT), n = n0 * 16 + col;
+        const int r = it / (16 * NT), col = it % (16 * NT), n = blockIdx.x * 16 * NT + col;
         if (n >= a.n) continue;
-        float y = 0.f;
+        float y = a.bias ? to_f(((const T *)a.bias)[n]) : 0.f;
+#pragma unroll 4
         for (int x = 0; x < waves; ++x) y += join[(x * rows + r) * LD + col];
-        if (a.bias) y += to_f(((const T *)a.bias)[n]);
         ((T *)a.y)[(int64_t)(m0 + r) * a.y_stride + n] = (T)y;
     }
 }
 
-template <class T, int MT, int NT, int GROUP> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
+template <class T, int NT, int GROUP> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
 {
-    constexpr int MAXW = MT == 1 ? 16 : 8;
-    const int chunks = (a.k + 127) / 128, blocks = (a.n + 16 * NT - 1) / (16 * NT), row_blocks = (a.m + 16 * MT - 1) / (16 * MT);
+    constexpr int MAXW = NT == 1 && sizeof(T) == 2 ? 16 : 8;
+    const int chunks = (a.k + 127) / 128, blocks = (a.n + 16 * NT - 1) / (16 * NT), row_blocks = (a.m + 15) / 16;
     // Waves share the chunks of k: eight, or sixteen where there are fewer workgroups than compute units.
     int waves = MAXW > 8 && blocks * row_blocks < 256 ? 16 : 8;
     while (waves > 1 && waves > chunks) waves /= 2;
-    const int rows = a.m < 16 * MT ? a.m : 16 * MT, bytes = waves * rows * (16 * NT + 1) * 4;
+    const int rows = a.m < 16 ? a.m : 16, bytes = waves * rows * (16 * NT + 1) * 4;
     static std::atomic<unsigned long long> done{0};
-    if (hipError_t e = ensure_dynamic_lds((const void *)linear_w4<T, MT, NT, GROUP, MAXW>, MAXW * 16 * MT * (16 * NT + 1) * 4, done)) return e;
-    linear_w4<T, MT, NT, GROUP, MAXW><<<dim3(blocks, row_blocks), waves * 64, bytes, st>>>(a);
+    if (hipError_t e = ensure_dynamic_lds((const void *)linear_w4<T, NT, GROUP, MAXW>, MAXW * 16 * (16 * NT + 1) * 4, done)) return e;
+    linear_w4<T, NT, GROUP, MAXW><<<dim3(blocks, row_blocks), waves * 64, bytes, st>>>(a);
     return hipSuccess;
 }
-template <class T, int MT, int NT> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
+template <class T, int NT> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
 {
-    return a.group == 32 ? start<T, MT, NT, 32>(a, st) : a.group == 64 ? start<T, MT, NT, 64>(a, st) : start<T, MT, NT, 128>(a, st);
-}
-template <class T, int MT> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
-{
-    return a.n >= 16 * 1024 ? start<T, MT, 2>(a, st) : start<T, MT, 1>(a, st);
+    return a.group == 32 ? start<T, NT, 32>(a, st) : a.group == 64 ? start<T, NT, 64>(a, st) : start<T, NT, 128>(a, st);
 }
 template <class T> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
 {
-    // Rows beyond 16 share the unpacked weights where the output tiles alone fill the chip; else they are workgroups of their own,
-    // which read the weights again from the cache.
-    const int tiles = (a.n + 15) / 16;
-    if (a.m <= 16 || tiles * ((a.m + 15) / 16) <= 512) return start<T, 1>(a, st);
-    return a.m <= 32 || tiles * ((a.m + 31) / 32) <= 512 ? start<T, 2>(a, st) : start<T, 4>(a, st);
+    // Every workgroup reads its rows of x whole: several output tiles a wave read them once, as long as the chip stays full and the
+    // registers hold (fp16, group 128: 8192 x 8192 with 16 rows 18.7 / 13.1 / 16.4 us at 1 / 2 / 4 tiles, with 64 rows 63 / 46 / 31 us;
+    // 4096 -> 2048, 32 rows: 6.8 / 7.6 / 9.0 us; bf16, group 32: 1024 -> 8192, 64 rows 15.2 / 12.9 / 16.1 us).
+    const int64_t tiles = (int64_t)((a.n + 15) / 16) * ((a.m + 15) / 16);
+    if (tiles < 512) return start<T, 1>(a, st);
+    if constexpr (sizeof(T) == 2)
+        if (tiles >= 1024 && a.group >= 64) return a.group == 64 ? start<T, 4, 64>(a, st) : start<T, 4, 128>(a, st);
+    return start<T, 2>(a, st);
 }
 
 }  // namespace

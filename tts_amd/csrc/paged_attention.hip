@@ -15,8 +15,8 @@ struct Launch {
     size_t part_bytes, stat_bytes;
 };
 
-// Waves of a workgroup, by what a wave's registers allow (128, 256 or 512 of them).
-constexpr int most_waves(int dp, int nq) { return dp == 64 && nq == 1 ? 16 : dp <= 128 ? 8 : 4; }
+// Waves of a workgroup, by what a wave's registers allow (256 or 512 of them).
+constexpr int most_waves(int dp) { return dp <= 128 ? 8 : 4; }
 
 // How a call is laid over the chip.  Sizes here are hints (max_new, max_len): the kernels compute whatever the device data holds.
 Launch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv &c, const ttsamd_paged_batch &b)
@@ -38,14 +38,18 @@ Launch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv &c, c
     const int64_t room = (int64_t)b.table_width * c.page_size;
     int64_t keys = b.max_len > 0 && b.max_len < room ? b.max_len : room;
     if (a.window > 0 && (int64_t)a.window + b.max_new < keys) keys = (int64_t)a.window + b.max_new;
-    const int kt = f32 || p.dp > 128 ? 16 : 32, most = most_waves(p.dp, p.nq);
+    const int kt = f32 || p.dp > 128 ? 16 : 32, most = most_waves(p.dp);
     const int64_t key_tiles = keys < 1 ? 1 : (keys + kt - 1) / kt, blocks = tiles * c.kv_heads * b.batch;
-    // Few workgroups: more waves to each, since they are joined in LDS for nothing but a barrier.
+    // Fewer workgroups than compute units: more waves to each, since they are joined in LDS for nothing but a barrier.  (One bf16 token of
+    // 16 heads over 605 keys: 2 / 4 / 8 waves 12.0 / 9.1 / 8.2 us; 2 x 437 fp32 tokens, 448 workgroups: 33.4 / 23.2 / 29.5 us.)
     p.waves = 4;
-    while (p.waves < most && blocks * p.waves < kCus * 8 && key_tiles > p.waves) p.waves *= 2;
-    // Still few, and long: the keys are split over workgroups, at least four tiles to a wave, and a second launch joins them.
+    while (p.waves < most && blocks < kCus && key_tiles > p.waves) p.waves *= 2;
+    // Still few, and long: the keys are split over workgroups until one round of them fills the registers of the chip, at least four
+    // tiles to a wave, and a second launch joins them.  (Three tokens over 65537 keys, 12 workgroups of 8 waves, one a compute unit:
+    // 21 / 32 / 42 / 85 splits 70.6 / 84.0 / 75.5 / 87.2 us.)
     p.splits = 1;
-    const int64_t fill = (int64_t)kCus * 16 / (blocks * p.waves), long_enough = key_tiles / (p.waves * 4);
+    const int resident = p.dp == 64 ? 12 : p.dp == 128 ? 8 : 4;        // waves a compute unit's registers hold
+    const int64_t fill = (int64_t)kCus * resident / (blocks * p.waves), long_enough = key_tiles / (p.waves * 4);
     if (fill > 1 && long_enough > 1) p.splits = (int)(fill < long_enough ? fill : long_enough);
     if ((int64_t)p.splits * c.kv_heads > 65535) p.splits = 65535 / c.kv_heads > 1 ? 65535 / c.kv_heads : 1;
     const int64_t each = (key_tiles + p.splits - 1) / p.splits;
@@ -59,7 +63,7 @@ Launch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv &c, c
 
 template <class T, int DP, int NQ, bool FULL> hipError_t start(const AttArgs &g, const Launch &p, dim3 grid, hipStream_t st)
 {
-    constexpr int MAXW = most_waves(DP, NQ);
+    constexpr int MAXW = most_waves(DP);
     static std::atomic<unsigned long long> done{0};
     const int bytes = p.waves * 16 * NQ * (DP + 4 + 2) * 4, most = MAXW * 16 * NQ * (DP + 4 + 2) * 4;
     if (hipError_t e = ensure_dynamic_lds((const void *)attend_stream<T, DP, NQ, FULL, MAXW>, most, done)) return e;

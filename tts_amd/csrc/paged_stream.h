@@ -120,6 +120,10 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
     const bool vrole = lane >= 32;
     const uint32_t page16 = (uint32_t)((vrole ? g.c.v_page : g.c.k_page) * ES / 16), row16 = (uint32_t)((vrole ? g.c.v_row : g.c.k_row) * ES / 16);
 
+    // the largest score is found before the scale: it has to be positive (a negative one turns q's sign, zero takes q away)
+    const unsigned flip = g.scale2 < 0.f ? F32 ? 0x80000000u : 0x80008000u : 0u, keep = g.scale2 == 0.f ? 0u : ~0u;
+    const float scale2 = g.scale2 == 0.f ? 1.f : fabsf(g.scale2);
+
     for (int r0 = blockIdx.y * 16 * NQ; r0 < rows; r0 += gridDim.y * 16 * NQ) {
         const int last = min(r0 + 16 * NQ, rows) - 1;
         Range mine[NQ];
@@ -133,6 +137,8 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
             for (int x = 0; x < NS; ++x) {
                 const int at = x * 64 + g4 * 16;
                 q[u][x] = FULL || at < D * ES ? *(const uint4 *)(src + (FULL || at < D * ES ? at : 0)) : uint4{0, 0, 0, 0};
+                q[u][x].x = (q[u][x].x & keep) ^ flip, q[u][x].y = (q[u][x].y & keep) ^ flip;
+                q[u][x].z = (q[u][x].z & keep) ^ flip, q[u][x].w = (q[u][x].w & keep) ^ flip;
             }
         }
         const Range first = seen_by(s, s.len - s.n + (int)g.by_group.div(r0), g.a.causal, g.a.window);
@@ -241,17 +247,17 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
             float p[NQ][VK];
 #pragma unroll
             for (int u = 0; u < NQ; ++u) {
-                unsigned dark = 0;                           // slots that this row does not see
                 if (!clear) {
 #pragma unroll
                     for (int e = 0; e < VK; ++e) {
                         const int kk = (e & 3) + 4 * g4 + (e >> 2) * 16, j = base + kk;
-                        if (!(ok_now >> kk & 1) || j < mine[u].begin || j >= mine[u].end) dark |= 1u << e;
+                        if (!(ok_now >> kk & 1) || j < mine[u].begin || j >= mine[u].end) sc[u][e >> 2][e & 3] = -INFINITY;
                     }
                 }
-                float top = kNoMax;
+                float top = sc[u][0][0];
 #pragma unroll
-                for (int e = 0; e < VK; ++e) top = fmaxf(top, !clear && (dark >> e & 1) ? kNoMax : sc[u][e >> 2][e & 3] * g.scale2);
+                for (int e = 1; e < VK; ++e) top = fmaxf(top, sc[u][e >> 2][e & 3]);
+                top *= scale2;
                 if (__any(top > m[u] + kLazy)) {
                     top = fmaxf(top, __shfl_xor(top, 16));
                     top = fmaxf(top, __shfl_xor(top, 32));
@@ -262,8 +268,7 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
                 }
 #pragma unroll
                 for (int e = 0; e < VK; ++e) {
-                    p[u][e] = __builtin_amdgcn_exp2f(fmaf(sc[u][e >> 2][e & 3], g.scale2, -m[u]));
-                    if (!clear && (dark >> e & 1)) p[u][e] = 0.f;
+                    p[u][e] = __builtin_amdgcn_exp2f(fmaf(sc[u][e >> 2][e & 3], scale2, -m[u]));
                     l[u] += p[u][e];
                 }
             }
@@ -330,34 +335,31 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
             }
         }
         __syncthreads();
-        const int cols = D / 8, nr = last - r0 + 1;
+        const int cols = D / 4, nr = last - r0 + 1, parts = redo ? 1 : waves;
         for (int w = threadIdx.x; w < nr * cols; w += blockDim.x) {
-            const int r = w / cols, d = (w - r * cols) * 8;
-            float top = kNoMax, sum = 0.f, acc[8] = {};
-            const int parts = redo ? 1 : waves;
+            const int r = w / cols, d = (w - r * cols) * 4;
+            float top = kNoMax, sum = 0.f;
+            f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
             for (int x = 0; x < parts; ++x) top = fmaxf(top, ml[2 * (x * R + r)]);
+#pragma unroll 4
             for (int x = 0; x < parts; ++x) {
                 const float f = __builtin_amdgcn_exp2f(ml[2 * (x * R + r)] - top);
                 sum += f * ml[2 * (x * R + r) + 1];
-                const float *src = lds + (x * R + r) * LDO + d;
-#pragma unroll
-                for (int y = 0; y < 8; ++y) acc[y] = fmaf(f, src[y], acc[y]);
+                acc += *(const f32x4_t *)(lds + (x * R + r) * LDO + d) * f;
             }
             const int row = r0 + r, i = g.by_group.div(row), h = hk * g.group + row - i * g.group;
             const int64_t token = s.start + i;
             if (g.splits > 1) {
                 const int64_t at = (token * g.a.q_heads + h) * g.splits + split;
-                *(f32x4_t *)(g.part + at * D + d) = f32x4_t{acc[0], acc[1], acc[2], acc[3]};
-                *(f32x4_t *)(g.part + at * D + d + 4) = f32x4_t{acc[4], acc[5], acc[6], acc[7]};
+                *(f32x4_t *)(g.part + at * D + d) = acc;
                 if (d == 0) g.stat[2 * at] = top, g.stat[2 * at + 1] = sum;
             } else {
-                alignas(16) T out[8];
                 const float inv = sum > 0.f ? 1.f / sum : sum;          // no key: zeros; NaN stays
-#pragma unroll
-                for (int y = 0; y < 8; ++y) out[y] = (T)(acc[y] * inv);
+                acc *= inv;
                 T *dst = (T *)g.a.out + token * g.a.o_tstride + (int64_t)h * g.a.o_hstride + d;
-#pragma unroll
-                for (int y = 0; y < 8 * ES / 16; ++y) ((uint4 *)dst)[y] = ((const uint4 *)out)[y];
+                if constexpr (F32) *(f32x4_t *)dst = acc;
+                else *(uint2 *)dst = uint2{pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3])};
             }
         }
     }
