@@ -859,20 +859,35 @@ _PACK_W4 = struct.Struct("PPqqPPPPiiiiii0q").pack
 _FNS = {}
 
 
-def _queue(what, device, *args):
-    """One call of the library's function `what` on the current stream of `device` (made current for the call if it is not)."""
+def _entry(what, arguments):
+    """The library's function `what`: a packed struct, then `arguments` pointers and sizes."""
     fn = _FNS.get(what)
     if fn is None:
         fn = getattr(lib(), "ttsamd_" + what)
-        fn.argtypes = [ctypes.c_char_p] + [ctypes.c_void_p] * (len(args) - 1) + [ctypes.c_void_p]
+        fn.argtypes = [ctypes.c_char_p] + [ctypes.c_void_p] * arguments
         _FNS[what] = fn
+    return fn
+
+
+def _queue(what, device, *args):
+    """One call of the library's function `what` on the current stream of `device` (made current for the call if it is not)."""
+    fn = _FNS.get(what) or _entry(what, len(args))
     index = device.index
-    if index != torch.cuda.current_device():
+    if index != _current_device():
         with torch.cuda.device(index):
-            return _queue(what, device, *args)
-    rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(*args, _current_stream(index))
+    else:
+        rc = fn(*args, _current_stream(index))
     if rc:
         check(rc, what)
+
+
+def _current_device():
+    return torch._C._cuda_getDevice()          # of a tensor that is on the GPU: the runtime is up
+
+
+def _current_stream(index):
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _rows(t, what, shape, dtype, device):
@@ -909,7 +924,6 @@ class Rotary:
 
     def __init__(self, head_dim, rotary_dim=None, base=10000.0, interleaved=False, scaling=None, inv_freq=None, amplitude=None, device="cuda"):
         import math
-        from fractions import Fraction
 
         rd = head_dim if rotary_dim is None else rotary_dim
         _need(rd % 2 == 0 and 0 <= rd <= head_dim, "rotary_dim %d of a head of %d: an even number up to it" % (rd, head_dim))
@@ -939,9 +953,14 @@ class Rotary:
         _need(all(math.isfinite(f) for f in freq), "a frequency is not finite")
         self.head_dim, self.rotary_dim, self.interleaved = head_dim, rd, bool(interleaved)
         self.amplitude = gain if amplitude is None else float(amplitude)
-        circle = 2 * Fraction(31415926535897932384626433832795028841971693993751, 10 ** 49)
-        turns = [round(Fraction(f) / circle * 2 ** 64) % 2 ** 64 for f in freq]
-        self.turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64).to(device)
+        # round(f / (2 pi) * 2^64) in whole numbers: f is a fraction, 2 pi one of fifty digits
+        top, bottom = 10 ** 49 << 64, 2 * 31415926535897932384626433832795028841971693993751
+        turns = []
+        for f in freq:
+            n, d = f.as_integer_ratio()
+            d *= bottom
+            turns.append((n * top + d // 2) // d + 2 ** 63 & 2 ** 64 - 1)
+        self.turns = torch.tensor([t - 2 ** 63 for t in turns], dtype=torch.int64).to(device)
         self.device = self.turns.device
         self._c = _RotaryPlan(self.turns.data_ptr() if rd else None, rd, int(self.interleaved), self.amplitude)
         self._ref = ctypes.addressof(self._c)
@@ -968,9 +987,11 @@ def rotary(plan, x, positions, out=None, inverse=False):
         _refuse("x has heads of %d channels, the plan of %d" % (dim, plan.head_dim))
     xt, xh = _rows(x, "x", shape, dtype, device)
     pp, pb = _positions(positions, tokens, device)
-    _lib.require_gpu(x, "x")
+    if not x.is_cuda:
+        _lib.require_gpu(x, "x")
     if out is None:
-        y, yt, yh = torch.empty(shape, dtype=dtype, device=device), heads * dim, dim
+        yt, yh = heads * dim, dim
+        y = torch.empty_like(x) if x.is_contiguous() else torch.empty(shape, dtype=dtype, device=device)
     else:
         y, (yt, yh) = out, _rows(out, "out", shape, dtype, device)
     _queue("rotary", device, _PACK_ROTARY(x.data_ptr(), y.data_ptr(), xt, xh, yt, yh, pp, pb, tokens, heads, dim, kind, 1 if inverse else 0), plan._ref)
@@ -994,6 +1015,7 @@ class PagedKV:
               "rows of the cache have to start at multiples of 16 bytes")
         self.k, self.v, self.dtype, self.device = k, v, k.dtype, k.device
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, rows, dim
+        self._scale = dim ** -0.5
         self._c = _PagedKV(k.data_ptr(), v.data_ptr(), *ks, *vs, _DTYPES[k.dtype], pages, heads, rows, dim)
         self._ref = ctypes.addressof(self._c)
 
@@ -1027,8 +1049,7 @@ class PagedBatch:
 
 
 def _same_device(batch, cache):
-    if batch.device != cache.device:
-        _refuse("the batch is on %s, the cache on %s" % (batch.device, cache.device))
+    _refuse("the batch is on %s, the cache on %s" % (batch.device, cache.device))
 
 
 def kv_append(cache, batch, k, v, rotary=None, q=None, positions=None, q_out=None):
@@ -1048,7 +1069,8 @@ def kv_append(cache, batch, k, v, rotary=None, q=None, positions=None, q_out=Non
             pp, pb = _positions(positions, tokens, device)
     elif positions is not None:
         _refuse("positions without a rotary plan")
-    _same_device(batch, cache)
+    if batch.device != device:
+        _same_device(batch, cache)
     if q is None:
         if q_out is not None:
             _refuse("q_out without q")
@@ -1060,9 +1082,11 @@ def kv_append(cache, batch, k, v, rotary=None, q=None, positions=None, q_out=Non
             _refuse("q is %s: [%d, q_heads, head_dim] is wanted" % (list(qs), tokens))
         qs = (tokens, qs[1], cache.head_dim)
         qt, qh = _rows(q, "q", qs, dtype, device)
-        _lib.require_gpu(k, "k")
+        if not k.is_cuda:
+            _lib.require_gpu(k, "k")
         if q_out is None:
-            q_out, ot, oh = torch.empty(qs, dtype=dtype, device=device), qs[1] * qs[2], qs[2]
+            ot, oh = qs[1] * qs[2], qs[2]
+            q_out = torch.empty_like(q) if q.is_contiguous() else torch.empty(qs, dtype=dtype, device=device)
         else:
             ot, oh = _rows(q_out, "q_out", qs, dtype, device)
         tail = (q.data_ptr(), q_out.data_ptr(), qt, qh, ot, oh, pp or 0, pb or 0, tokens, qs[1])
@@ -1083,13 +1107,16 @@ def paged_attention(q, cache, batch, scale=None, causal=True, window=0, out=None
     qt, qh = _rows(q, "q", shape, dtype, device)
     if not 0 <= window < 2 ** 31:
         _refuse("window %d" % window)
-    _same_device(batch, cache)
-    _lib.require_gpu(q, "q")
+    if batch.device != device:
+        _same_device(batch, cache)
+    if not q.is_cuda:
+        _lib.require_gpu(q, "q")
     if out is None:
-        o, ot, oh = torch.empty(shape, dtype=dtype, device=device), shape[1] * dim, dim
+        ot, oh = shape[1] * dim, dim
+        o = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dtype, device=device)
     else:
         o, (ot, oh) = out, _rows(out, "out", shape, dtype, device)
-    a = _PACK_ATTENTION(q.data_ptr(), o.data_ptr(), qt, qh, ot, oh, shape[0], shape[1], 1 if causal else 0, window, dim ** -0.5 if scale is None else scale)
+    a = _PACK_ATTENTION(q.data_ptr(), o.data_ptr(), qt, qh, ot, oh, shape[0], shape[1], 1 if causal else 0, window, cache._scale if scale is None else scale)
     need = _workspace_bytes()(a, cache._ref, batch._ref)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _queue("paged_attention", device, a, cache._ref, batch._ref, ws.data_ptr() if need else None, need)
@@ -1097,11 +1124,7 @@ def paged_attention(q, cache, batch, scale=None, causal=True, window=0, out=None
 
 
 def _workspace_bytes():
-    fn = _FNS.get("workspace")
-    if fn is None:
-        fn = _FNS["workspace"] = lib().ttsamd_paged_attention_workspace_bytes
-        fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_void_p]
-    return fn
+    return _FNS.get("paged_attention_workspace_bytes") or _entry("paged_attention_workspace_bytes", 2)
 
 
 class PackedW4:
@@ -1178,10 +1201,11 @@ def linear_w4(weights, x, out=None):
         _refuse("the channels of a row of x have to be contiguous")
     if x.device != device or w.bias_dtype not in (None, dtype):
         _refuse("x is %s on %s, the layer %s on %s" % (dtype, x.device, w.bias_dtype or dtype, device))
-    _lib.require_gpu(x, "x")
+    if not x.is_cuda:
+        _lib.require_gpu(x, "x")
     m, n = shape[0], w.n
     if out is None:
-        y, ys = torch.empty((m, n), dtype=dtype, device=device), n
+        y, ys = x.new_empty((m, n)), n
     else:
         y = out
         if y.shape != (m, n) or y.dtype != dtype or y.device != device or (y.stride(1) != 1 and n > 1):
