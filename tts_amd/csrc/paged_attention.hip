@@ -26,31 +26,30 @@ Launch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv &c, c
     const int group = a.q_heads / c.kv_heads;
     p.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
     const int64_t rows = (int64_t)(b.max_new < 1 ? 1 : b.max_new) * group;
-    const int64_t tile_blocks = (rows + kTileRows - 1) / kTileRows * c.kv_heads * b.batch;
-    if (!f32 && rows >= 64 && tile_blocks >= 64) {
-        p.tile = true, p.splits = 1;
-        p.row_tiles = (int)((rows + kTileRows - 1) / kTileRows < 65535 ? (rows + kTileRows - 1) / kTileRows : 65535);
-        return p;
-    }
+    // Rows enough for the staged kernel, by type and row: 4096 keys, one sequence, 128 / 256 / 512 / 1024 rows of 8 key heads of 128: streamed
+    // 26 / 30 / 39 / 57 us, staged 30 / 33 / 41 / 50; of 16 of 64: 21 / 35 / 48 us (128 / 256 / 512 rows), staged 21 / 25 / 29.
+    p.tile = !f32 && rows >= 256;
     p.nq = rows > 16 && p.dp < 256 ? 2 : 1;
-    const int64_t tiles = (rows + 16 * p.nq - 1) / (16 * p.nq);
+    const int block_rows = p.tile ? kTileRows : 16 * p.nq, kt = p.tile ? kTileKeys : f32 || p.dp > 128 ? 16 : 32;
+    const int64_t tiles = (rows + block_rows - 1) / block_rows;
     p.row_tiles = (int)(tiles < 65535 ? tiles : 65535);
     const int64_t room = (int64_t)b.table_width * c.page_size;
     int64_t keys = b.max_len > 0 && b.max_len < room ? b.max_len : room;
     if (a.window > 0 && (int64_t)a.window + b.max_new < keys) keys = (int64_t)a.window + b.max_new;
-    const int kt = f32 || p.dp > 128 ? 16 : 32, most = most_waves(p.dp);
     const int64_t key_tiles = keys < 1 ? 1 : (keys + kt - 1) / kt, blocks = tiles * c.kv_heads * b.batch;
     // Fewer workgroups than compute units: more waves to each, since they are joined in LDS for nothing but a barrier.  (One bf16 token of
     // 16 heads over 605 keys: 2 / 4 / 8 waves 12.0 / 9.1 / 8.2 us; 2 x 437 fp32 tokens, 448 workgroups: 33.4 / 23.2 / 29.5 us.)
     p.waves = 4;
-    while (p.waves < most && blocks < kCus && key_tiles > p.waves) p.waves *= 2;
-    // Still few, and long: the keys are split over workgroups until one round of them fills the registers of the chip, at least four
-    // tiles to a wave, and a second launch joins them.  (Three tokens over 65537 keys, 12 workgroups of 8 waves, one a compute unit:
-    // 21 / 32 / 42 / 85 splits 70.6 / 84.0 / 75.5 / 87.2 us.)
+    while (!p.tile && p.waves < most_waves(p.dp) && blocks < kCus && key_tiles > p.waves) p.waves *= 2;
+    // Still few, and long: the keys are split over workgroups until one round of them fills the chip, and a second launch joins them.
+    // (Three tokens over 65537 keys, 12 workgroups of 8 waves, one a compute unit: 21 / 32 / 42 / 85 splits 70.6 / 84.0 / 75.5 / 87.2 us;
+    // one bf16 token over 605 keys, 2.4 tiles a wave: whole 8.2 us, two splits 11.0; one over 4096, 16 tiles a wave: at least 1 / 2 / 4
+    // tiles left to a wave 14.1 / 16.0 / 21.0 us.)
     p.splits = 1;
-    const int resident = p.dp == 64 ? 12 : p.dp == 128 ? 8 : 4;        // waves a compute unit's registers hold
-    const int64_t fill = (int64_t)kCus * resident / (blocks * p.waves), long_enough = key_tiles / (p.waves * 4);
-    if (fill > 1 && long_enough > 1) p.splits = (int)(fill < long_enough ? fill : long_enough);
+    const int resident = (p.dp > 128 ? 4 : p.dp == 64 && !p.tile ? 12 : 8) / p.waves;    // workgroups a compute unit's registers hold
+    const int64_t fill = (int64_t)kCus * (resident < 1 ? 1 : resident) / blocks, a_wave = p.tile ? 1 : p.waves;
+    const int64_t most = key_tiles / (a_wave * (p.tile || rows > 64 ? 4 : rows > 32 ? 2 : 1));       // tiles left to a wave: the join costs by the row
+    if (fill > 1 && key_tiles > 4 * a_wave) p.splits = (int)(fill < most ? fill : most);
     if ((int64_t)p.splits * c.kv_heads > 65535) p.splits = 65535 / c.kv_heads > 1 ? 65535 / c.kv_heads : 1;
     const int64_t each = (key_tiles + p.splits - 1) / p.splits;
     p.split_keys = (int)(each * kt < 0x7fffffff ? each * kt : 0x7fffffff);
@@ -89,7 +88,7 @@ template <class T, int DP> hipError_t start_tile(const AttArgs &g, dim3 grid, hi
 template <class T> hipError_t start(const AttArgs &g, const Launch &p, hipStream_t st)
 {
     if constexpr (sizeof(T) == 2) {
-        const dim3 grid(g.c.kv_heads, p.row_tiles, g.b.batch);
+        const dim3 grid(g.c.kv_heads * p.splits, p.row_tiles, g.b.batch);
         if (p.tile) return p.dp == 64 ? start_tile<T, 64>(g, grid, st) : p.dp == 128 ? start_tile<T, 128>(g, grid, st) : start_tile<T, 256>(g, grid, st);
     }
     const dim3 grid(g.c.kv_heads * p.splits, p.row_tiles, g.b.batch);
@@ -99,8 +98,13 @@ template <class T> hipError_t start(const AttArgs &g, const Launch &p, hipStream
 }
 template <class T> void join(const AttArgs &g, hipStream_t st)
 {
-    const int n = g.b.max_new < 1 ? 1 : g.b.max_new;
-    join_splits<T><<<dim3(n < 65536 ? n : 65536, g.a.q_heads, g.b.batch), 256, 0, st>>>(g);
+    // a quarter of the splits to a lane, as long as a row's lanes fit a workgroup
+    const int cols = g.c.head_dim / 8, n = g.b.max_new < 1 ? 1 : g.b.max_new;
+    int lanes = 1;
+    while (lanes * 4 < g.splits && lanes * 2 * cols <= 256) lanes *= 2;
+    const int teams = 256 / (cols * lanes);
+    const int64_t blocks = ((int64_t)n * g.a.q_heads + teams - 1) / teams;
+    join_splits<T><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536), g.b.batch), 256, 0, st>>>(g, lanes);
 }
 
 int check(const ttsamd_paged_attention_args *a, const ttsamd_paged_kv *cache, const ttsamd_paged_batch *batch)

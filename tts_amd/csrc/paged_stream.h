@@ -365,50 +365,58 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
     }
 }
 
-// Joins the splits of one (token, head): a thread owns eight channels of every 256 / (head_dim / 8)-th split, LDS adds them up.
-template <class T> __global__ __launch_bounds__(256) void join_splits(AttArgs g)
+// Joins the splits: a thread owns eight channels of a row (token, head) and every lanes-th split of it; the lanes of a row are added
+// up in LDS, in their order.  lanes: a power of two, lanes * head_dim / 8 <= 256.
+template <class T> __global__ __launch_bounds__(256) void join_splits(AttArgs g, int lanes)
 {
     constexpr int ES = sizeof(T);
     __shared__ float lds[256 * 9];
-    const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, blockIdx.z);
-    const int D = g.c.head_dim, cols = D / 8, lanes = 256 / cols, h = blockIdx.y;
-    const int at_col = threadIdx.x % cols, at_lane = threadIdx.x / cols, d = at_col * 8;
-    for (int i = blockIdx.x; i < s.n; i += gridDim.x) {
-        const int64_t token = s.start + i, at = (token * g.a.q_heads + h) * g.splits;
-        float top = kNoMax, sum = 0.f, acc[8] = {};
-        if (at_lane < lanes) {
-            for (int x = at_lane; x < g.splits; x += lanes) top = fmaxf(top, g.stat[2 * (at + x)]);
-            for (int x = at_lane; x < g.splits; x += lanes) {
+    const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, blockIdx.y);
+    const int D = g.c.head_dim, cols = D / 8, team = cols * lanes, teams = 256 / team;
+    const int mine = threadIdx.x / team, in_team = threadIdx.x - mine * team, lane = in_team / cols, col = in_team - lane * cols, d = col * 8;
+    const int64_t rows = (int64_t)s.n * g.a.q_heads;
+    for (int64_t r0 = (int64_t)blockIdx.x * teams; r0 < rows; r0 += (int64_t)gridDim.x * teams) {
+        const int64_t row = r0 + mine;
+        const bool in = mine < teams && row < rows;
+        const int64_t at = ((int64_t)s.start * g.a.q_heads + row) * g.splits;
+        float top = kNoMax, all[9] = {};
+        if (in) {
+            for (int x = lane; x < g.splits; x += lanes) top = fmaxf(top, g.stat[2 * (at + x)]);
+#pragma unroll 2
+            for (int x = lane; x < g.splits; x += lanes) {
                 const float f = __builtin_amdgcn_exp2f(g.stat[2 * (at + x)] - top);
-                sum += f * g.stat[2 * (at + x) + 1];
                 const f32x4_t a0 = *(const f32x4_t *)(g.part + (at + x) * D + d), a1 = *(const f32x4_t *)(g.part + (at + x) * D + d + 4);
 #pragma unroll
-                for (int y = 0; y < 4; ++y) acc[y] = fmaf(f, a0[y], acc[y]), acc[4 + y] = fmaf(f, a1[y], acc[4 + y]);
+                for (int y = 0; y < 4; ++y) all[y] = fmaf(f, a0[y], all[y]), all[4 + y] = fmaf(f, a1[y], all[4 + y]);
+                all[8] = fmaf(f, g.stat[2 * (at + x) + 1], all[8]);
             }
         }
-        // each has a maximum of its own: brought to the largest, then added in the order of the lanes
-        float *const mine = lds + threadIdx.x * 9;
-        __syncthreads();
-        mine[8] = top;
-        __syncthreads();
-        float best = top;
-        for (int x = 0; x < lanes; ++x) best = fmaxf(best, lds[(x * cols + at_col) * 9 + 8]);
-        const float f = __builtin_amdgcn_exp2f(top - best);
-        __syncthreads();
+        if (lanes > 1) {
+            // each lane has a maximum of its own: brought to the largest first
+            const int base = mine * team + col;
+            __syncthreads();
+            lds[threadIdx.x * 9 + 8] = top;
+            __syncthreads();
+            float best = top;
+            if (in)
+                for (int x = 0; x < lanes; ++x) best = fmaxf(best, lds[(base + x * cols) * 9 + 8]);
+            const float f = __builtin_amdgcn_exp2f(top - best);
+            __syncthreads();
 #pragma unroll
-        for (int y = 0; y < 8; ++y) mine[y] = acc[y] * f;
-        mine[8] = sum * f;
-        __syncthreads();
-        if (at_lane == 0) {
-            float all[9] = {};
-            for (int x = 0; x < lanes; ++x)
+            for (int y = 0; y < 9; ++y) lds[threadIdx.x * 9 + y] = all[y] * f, all[y] = 0.f;
+            __syncthreads();
+            if (in && lane == 0)
+                for (int x = 0; x < lanes; ++x)
 #pragma unroll
-                for (int y = 0; y < 9; ++y) all[y] += lds[(x * cols + at_col) * 9 + y];
+                    for (int y = 0; y < 9; ++y) all[y] += lds[(base + x * cols) * 9 + y];
+        }
+        if (in && lane == 0) {
             alignas(16) T out[8];
             const float inv = all[8] > 0.f ? 1.f / all[8] : all[8];
 #pragma unroll
             for (int y = 0; y < 8; ++y) out[y] = (T)(all[y] * inv);
-            T *dst = (T *)g.a.out + token * g.a.o_tstride + (int64_t)h * g.a.o_hstride + d;
+            const int64_t token = s.start + row / g.a.q_heads;
+            T *dst = (T *)g.a.out + token * g.a.o_tstride + (row % g.a.q_heads) * g.a.o_hstride + d;
 #pragma unroll
             for (int y = 0; y < 8 * ES / 16; ++y) ((uint4 *)dst)[y] = ((const uint4 *)out)[y];
         }

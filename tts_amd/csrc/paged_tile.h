@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
     extern __shared__ float lds_f[];
     char *const lds = (char *)lds_f;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c32 = lane & 31, h2 = lane >> 5;
-    const int hk = blockIdx.x, b = blockIdx.z;
+    const int hk = blockIdx.x / g.splits, split = blockIdx.x - hk * g.splits, b = blockIdx.z;
     const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, b);
     const int D = g.c.head_dim, rows = s.n * g.group, tiles = (rows + kTileRows - 1) / kTileRows;
     const char *kbase = (const char *)g.c.k + (int64_t)hk * g.c.k_head * 2, *vbase = (const char *)g.c.v + (int64_t)hk * g.c.v_head * 2;
@@ -83,7 +83,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
         float m = kNoMax, l = 0.f;
         bool odd = false;
 
-        const int lo = first.begin, hi = final.end;
+        const int64_t from = first.begin + (int64_t)split * g.split_keys, to = split + 1 < g.splits ? from + g.split_keys : final.end;
+        const int lo = (int)min(from, (int64_t)final.end), hi = (int)min(to, (int64_t)final.end);
         uint4 st[NSTG];                                      // what travels: keys first, then values
         auto fetch = [&](int at, int &row) {
             const int j = at + lane;
@@ -214,28 +215,38 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
         const bool redo = __syncthreads_or(odd);
         if (!redo) {
             l += __shfl_xor(l, 32);
-            const float inv = l > 0.f ? 1.f / l : l;          // no key: zeros; NaN stays
             if (r0 + 32 * wave + c32 <= last) {
-                T *dst = (T *)g.a.out + (int64_t)(s.start + my_i) * g.a.o_tstride + (int64_t)my_h * g.a.o_hstride;
+                const int64_t token = s.start + my_i, at = (token * g.a.q_heads + my_h) * g.splits + split;
+                const float inv = l > 0.f ? 1.f / l : l;      // no key: zeros; NaN stays
+                T *dst = (T *)g.a.out + token * g.a.o_tstride + (int64_t)my_h * g.a.o_hstride;
 #pragma unroll
                 for (int x = 0; x < ND; ++x)
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
                         const int d = 32 * x + 8 * y + 4 * h2;
-                        if (FULL || d < D)
-                            *(uint2 *)(dst + d) = uint2{pack2<T>(o[x][4 * y] * inv, o[x][4 * y + 1] * inv), pack2<T>(o[x][4 * y + 2] * inv, o[x][4 * y + 3] * inv)};
+                        if (!FULL && d >= D) continue;
+                        const f32x4_t v = {o[x][4 * y], o[x][4 * y + 1], o[x][4 * y + 2], o[x][4 * y + 3]};
+                        if (g.splits > 1) *(f32x4_t *)(g.part + at * D + d) = v;
+                        else *(uint2 *)(dst + d) = uint2{pack2<T>(v[0] * inv, v[1] * inv), pack2<T>(v[2] * inv, v[3] * inv)};
                     }
+                if (g.splits > 1 && h2 == 0) g.stat[2 * at] = m, g.stat[2 * at + 1] = l;
             }
         } else {
             float *const mine_o = lds_f + wave * 264;
             for (int r = r0 + wave; r <= last; r += 4) {
                 const int i = g.by_group.div(r), h = hk * g.group + r - i * g.group;
-                const int64_t token = s.start + i;
-                const float sum = attend_row<T>(g, b, hk, (const T *)g.a.q + token * g.a.q_tstride + (int64_t)h * g.a.q_hstride, range_of(r), mine_o,
+                const int64_t token = s.start + i, at = (token * g.a.q_heads + h) * g.splits + split;
+                Range see = range_of(r);
+                see.begin = max(see.begin, lo), see.end = min(see.end, hi);
+                const float sum = attend_row<T>(g, b, hk, (const T *)g.a.q + token * g.a.q_tstride + (int64_t)h * g.a.q_hstride, see, mine_o,
                                                 mine_o + 256);
                 const float inv = sum > 0.f ? 1.f / sum : sum;
                 T *dst = (T *)g.a.out + token * g.a.o_tstride + (int64_t)h * g.a.o_hstride;
-                for (int d = lane; d < D; d += 64) dst[d] = (T)(mine_o[d] * inv);
+                for (int d = lane; d < D; d += 64) {
+                    if (g.splits > 1) g.part[at * D + d] = mine_o[d];
+                    else dst[d] = (T)(mine_o[d] * inv);
+                }
+                if (g.splits > 1 && lane == 0) g.stat[2 * at] = mine_o[256], g.stat[2 * at + 1] = sum;
             }
         }
     }
