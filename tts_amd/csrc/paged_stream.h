@@ -76,6 +76,20 @@ template <class T> __device__ __forceinline__ bool any_odd(unsigned w)
     else return (w & X) == X || (w >> 16 & X) == X;
 }
 
+// Which of the 64 keys from `base` a row sees.
+__device__ __forceinline__ uint64_t seen_bits(uint64_t ok, int base, Range see)
+{
+    const int from = max(see.begin - base, 0), to = see.end - base;
+    if (from >= 64 || to <= from) return 0;
+    return ok & (~0ull << from) & (to >= 64 ? ~0ull : ~(~0ull << to));
+}
+// x where bit `b` of `bits` is set, else minus infinity.
+__device__ __forceinline__ float masked(float x, uint32_t bits, int b)
+{
+    const uint32_t all = (uint32_t)((int32_t)(bits << (31 - b)) >> 31);
+    return __uint_as_float((__float_as_uint(x) & all) | (0xff800000u & ~all));
+}
+
 // One row's keys [lo, hi), a wave, key by key: o[d] += p v only for the keys of `see`.  For the rare tile where a value that some row
 // must not see is an infinity or NaN.  Lane x owns o[x], o[x + 64], ..; returns the sum of the p (every lane).
 template <class T>
@@ -248,11 +262,9 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
 #pragma unroll
             for (int u = 0; u < NQ; ++u) {
                 if (!clear) {
+                    const uint32_t bits = (uint32_t)seen_bits(ok_now, base, mine[u]) >> (4 * g4);
 #pragma unroll
-                    for (int e = 0; e < VK; ++e) {
-                        const int kk = (e & 3) + 4 * g4 + (e >> 2) * 16, j = base + kk;
-                        if (!(ok_now >> kk & 1) || j < mine[u].begin || j >= mine[u].end) sc[u][e >> 2][e & 3] = -INFINITY;
-                    }
+                    for (int e = 0; e < VK; ++e) sc[u][e >> 2][e & 3] = masked(sc[u][e >> 2][e & 3], bits, (e & 3) + (e >> 2) * 16);
                 }
                 float top = sc[u][0][0];
 #pragma unroll

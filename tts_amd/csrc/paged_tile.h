@@ -36,7 +36,7 @@ constexpr int kTileRows = 128, kTileKeys = 64;
 template <class T, int DP, bool FULL>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
 {
-    constexpr int CH = DP / 8, RB = DP * 2, NSTG = CH / 4, RPI = 64 / CH, NS = DP / 16, ND = DP / 32;
+    constexpr int CH = DP / 8, RB = DP * 2, NSTG = CH / 4, RPI = 64 / CH, NS = DP / 16, ND = DP / 32, AHEAD = 4;
     constexpr int HALF = kTileKeys * RB;                    // bytes of a tile's keys (or values)
     extern __shared__ float lds_f[];
     char *const lds = (char *)lds_f;
@@ -151,17 +151,22 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
             f32x16_t sc[2];
             if (busy) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    f32x16_t acc;
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int y = 0; y < 16; ++y) acc[y] = 0.f;
-                    const int r = 32 * t + c32;
-                    const char *kr = kb + r * RB;
+                    for (int y = 0; y < 16; ++y) sc[t][y] = 0.f;
+                const char *kr = kb + c32 * RB;
+                const int kswz = k_swz(c32);                 // rows 32 apart are permuted alike
+                auto k_piece = [&](int i) { return *(const uint4 *)(kr + (i & 1) * 32 * RB + (((i & ~1) + h2) ^ kswz) * 16); };
+                uint4 kf[AHEAD];
 #pragma unroll
-                    for (int x = 0; x < NS; ++x)
-                        acc = mfma_32x32x16<T>(*(const uint4 *)(kr + (((2 * x + h2) ^ k_swz(r)) & (CH - 1)) * 16), q[x], acc);
-                    sc[t] = acc;
+                for (int i = 0; i < AHEAD; ++i) kf[i] = k_piece(i);
+#pragma unroll
+                for (int i = 0; i < 2 * NS; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);       // in this order: the reads stay AHEAD products ahead
+                    sc[i & 1] = mfma_32x32x16<T>(kf[i % AHEAD], q[i >> 1], sc[i & 1]);
+                    if (i + AHEAD < 2 * NS) kf[i % AHEAD] = k_piece(i + AHEAD);
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             if (more) {
                 put_k(next);
@@ -170,11 +175,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
             if (busy) {
                 // slot y of half h2 of tile t: key 32 t + 8 (y / 4) + 4 h2 + y % 4
                 if (ok_now != ~0ull || base < wlast.begin || base + kTileKeys > wfirst.end) {
+                    const uint64_t bits = seen_bits(ok_now, base, mine) >> (4 * h2);
 #pragma unroll
-                    for (int y = 0; y < 32; ++y) {
-                        const int kk = 32 * (y >> 4) + 8 * (y >> 2 & 3) + 4 * h2 + (y & 3), j = base + kk;
-                        if (!(ok_now >> kk & 1) || j < mine.begin || j >= mine.end) sc[y >> 4][y & 15] = -INFINITY;
-                    }
+                    for (int y = 0; y < 32; ++y) sc[y >> 4][y & 15] = masked(sc[y >> 4][y & 15], (uint32_t)(bits >> (y & 16 ? 32 : 0)), 8 * (y >> 2 & 3) + (y & 3));
                 }
                 float top = sc[0][0];
 #pragma unroll
@@ -187,27 +190,42 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
 #pragma unroll
                     for (int x = 0; x < ND; ++x) o[x] *= fade;
                 }
+                typedef short s4 __attribute__((ext_vector_type(4)));
+                const char *vrow = vb + vr * RB + vb8;
+                const int vswz = v_swz(vr);                  // rows four apart are permuted alike
+                // the left operand of product i = u * ND + x: sixteen keys of 32 channels
+                auto v_piece = [&](int i) {
+                    const char *at = vrow + 16 * (i / ND) * RB + ((4 * (i % ND) + vc) ^ vswz) * 16;
+                    const uint2 lower = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)at));
+                    const uint2 upper = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(at + 8 * RB)));
+                    return uint4{lower.x, lower.y, upper.x, upper.y};
+                };
+                // two of a group's eight probabilities, rounded
+                auto p_pair = [&](int u, int y) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[u >> 1][(u & 1) * 8 + 2 * y], scale2, -m));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[u >> 1][(u & 1) * 8 + 2 * y + 1], scale2, -m));
+                    return pack2<T>(p0, p1);
+                };
+                unsigned pb[2][4];
+                uint4 vf[AHEAD];
 #pragma unroll
-                for (int y = 0; y < 32; ++y) sc[y >> 4][y & 15] = __builtin_amdgcn_exp2f(fmaf(sc[y >> 4][y & 15], scale2, -m));
+                for (int i = 0; i < AHEAD; ++i) vf[i] = v_piece(i);
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const f32x16_t &p = sc[u >> 1];
-                    const int y = (u & 1) * 8;
-                    const uint4 pb = {pack2<T>(p[y], p[y + 1]), pack2<T>(p[y + 2], p[y + 3]), pack2<T>(p[y + 4], p[y + 5]), pack2<T>(p[y + 6], p[y + 7])};
-                    l = sum2<T>(pb.x, sum2<T>(pb.y, sum2<T>(pb.z, sum2<T>(pb.w, l))));
+                for (int y = 0; y < 4; ++y) pb[0][y] = p_pair(0, y);
 #pragma unroll
-                    for (int x = 0; x < ND; ++x) {
-                        typedef short s4 __attribute__((ext_vector_type(4)));
-                        uint2 part[2];
+                for (int i = 0; i < 4 * ND; ++i) {
+                    const int u = i / ND, x = i % ND;
+                    __builtin_amdgcn_sched_barrier(0);
+                    o[x] = mfma_32x32x16<T>(vf[i % AHEAD], uint4{pb[u & 1][0], pb[u & 1][1], pb[u & 1][2], pb[u & 1][3]}, o[x]);
+                    if (i + AHEAD < 4 * ND) vf[i % AHEAD] = v_piece(i + AHEAD);
+                    // while it runs: a share of the next group's probabilities, and this one's sum
 #pragma unroll
-                        for (int z = 0; z < 2; ++z) {
-                            const int r = 16 * u + 8 * z + vr;
-                            const char *at = vb + r * RB + (((4 * x + vc) ^ v_swz(r)) & (CH - 1)) * 16 + vb8;
-                            part[z] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)at));
-                        }
-                        o[x] = mfma_32x32x16<T>(uint4{part[0].x, part[0].y, part[1].x, part[1].y}, pb, o[x]);
+                    for (int y = x * 4 / ND; y < (x + 1) * 4 / ND; ++y) {
+                        if (u < 3) pb[(u + 1) & 1][y] = p_pair(u + 1, y);
+                        l = sum2<T>(pb[u & 1][y], l);
                     }
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             if (more) put_v(next, ok, mixed_at(base + kTileKeys, ok));
             cur ^= 1;
