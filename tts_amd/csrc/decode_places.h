@@ -52,13 +52,21 @@ TTSAMD_HD Range seen_by(const Sequence &s, int pos, int causal, int window)
     return Range{window > 0 && from > 0 ? (int)from : 0, causal && pos + 1 < s.keys ? (pos + 1 < 0 ? 0 : pos + 1) : s.keys};
 }
 
-// The page of sequence b that holds position j in [0, s.keys), or -1; `row`: the row in it.
-TTSAMD_HD int page_of(const ttsamd_paged_batch &bt, const FastDiv &by_page, int pages, int b, int j, int &row)
+// The table's entry for position j of sequence b, j in [0, s.keys), and the row in its page.  What the entry holds is checked where it is
+// used (held), so that a kernel can leave the load on its way.
+TTSAMD_HD int entry_of(const ttsamd_paged_batch &bt, const FastDiv &by_page, int b, int j, int &row)
 {
     const uint32_t col = by_page.div((uint32_t)j);
     row = j - (int)(col * by_page.d);
-    const int page = bt.block_table[b * bt.table_stride + col];
-    return (unsigned)page < (unsigned)pages ? page : -1;
+    return bt.block_table[b * bt.table_stride + col];
+}
+TTSAMD_HD bool held(int page, int pages) { return (unsigned)page < (unsigned)pages; }
+
+// The page of sequence b that holds position j in [0, s.keys), or -1; `row`: the row in it.
+TTSAMD_HD int page_of(const ttsamd_paged_batch &bt, const FastDiv &by_page, int pages, int b, int j, int &row)
+{
+    const int page = entry_of(bt, by_page, b, j, row);
+    return held(page, pages) ? page : -1;
 }
 
 }  // namespace ttsamd

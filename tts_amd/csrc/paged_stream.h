@@ -175,12 +175,9 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
         const int step = waves * KT, idx = lane & (KT - 1);
         uint4 k[NT][NS];
         unsigned v[VK][VB / 4];
-        // place of this lane's key of the tile at `at`: the table's page, -1 where the key is not one of [lo, hi)
-        auto fetch = [&](int at, int &row) {
-            const int j = at + idx;
-            row = 0;
-            return j < hi ? page_of(g.b, g.by_page, g.c.pages, b, j, row) : -1;
-        };
+        // the table's entry for this lane's key of the tile at `at`, still on its way; what it is worth once it is there
+        auto fetch = [&](int at, int &row) { return entry_of(g.b, g.by_page, b, min(at + idx, hi - 1), row); };
+        auto place = [&](int at, int entry) { return at + idx < hi && held(entry, g.c.pages) ? entry : -1; };
         auto load_k = [&](uint32_t off) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -198,7 +195,7 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
         unsigned ok = 0;
         if (base < hi) {
             int row;
-            const int page = fetch(base, row);
+            const int page = place(base, fetch(base, row));
             off = page < 0 ? 0 : (uint32_t)page * page16 + (uint32_t)row * row16;
             ok = (unsigned)__ballot(page >= 0) & (KT == 32 ? ~0u : 0xffffu);
             load_k(off);
@@ -222,8 +219,9 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
                 }
             }
             const unsigned ok_now = ok;
-            off = page_next < 0 ? 0 : (uint32_t)page_next * page16 + (uint32_t)row_next * row16;
-            ok = (unsigned)__ballot(page_next >= 0) & (KT == 32 ? ~0u : 0xffffu);
+            const int page = place(base + step, page_next);
+            off = page < 0 ? 0 : (uint32_t)page * page16 + (uint32_t)row_next * row16;
+            ok = (unsigned)__ballot(page >= 0) & (KT == 32 ? ~0u : 0xffffu);
             page_next = fetch(base + 2 * step, row_next);
 
             f32x4_t sc[NQ][NT];

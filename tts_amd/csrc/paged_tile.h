@@ -86,11 +86,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
         const int64_t from = first.begin + (int64_t)split * g.split_keys, to = split + 1 < g.splits ? from + g.split_keys : final.end;
         const int lo = (int)min(from, (int64_t)final.end), hi = (int)min(to, (int64_t)final.end);
         uint4 st[NSTG];                                      // what travels: keys first, then values
-        auto fetch = [&](int at, int &row) {
-            const int j = at + lane;
-            row = 0;
-            return j < hi ? page_of(g.b, g.by_page, g.c.pages, b, j, row) : -1;
-        };
+        // the table's entry for this lane's key of the tile at `at`, still on its way; what it is worth once it is there
+        auto fetch = [&](int at, int &row) { return entry_of(g.b, g.by_page, b, min(at + lane, hi - 1), row); };
+        auto place = [&](int at, int entry) { return at + lane < hi && held(entry, g.c.pages) ? entry : -1; };
         auto stage = [&](const char *src, uint32_t off) {
 #pragma unroll
             for (int x = 0; x < NSTG; ++x) st[x] = *(const uint4 *)(src + (uint64_t)(uint32_t)__shfl((int)off, (x * 4 + wave) * RPI + row_of_lane) * 16);
@@ -127,7 +125,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
         __syncthreads();                                     // the last row tile's readers are done
         if (lo < hi) {
             int row;
-            const int page = fetch(lo, row);
+            const int page = place(lo, fetch(lo, row));
             ok = __ballot(page >= 0);
             page_next = fetch(lo + kTileKeys, row_next);
             stage(kbase_l, k_off(page, row));
@@ -143,9 +141,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
             const bool more = base + kTileKeys < hi, busy = base < wlast.end && base + kTileKeys > wfirst.begin;
             uint32_t voff = 0;
             if (more) {
-                ok = __ballot(page_next >= 0);
-                stage(kbase_l, k_off(page_next, row_next));
-                voff = v_off(page_next, row_next);
+                const int page = place(base + kTileKeys, page_next);
+                ok = __ballot(page >= 0);
+                stage(kbase_l, k_off(page, row_next));
+                voff = v_off(page, row_next);
                 page_next = fetch(base + 2 * kTileKeys, row_next);
             }
             f32x16_t sc[2];
