@@ -387,3 +387,160 @@ def test_quantize_is_within_half_a_step(gpu, group, zeros):
     step = (f.amax(-1).clamp(min=0) - f.amin(-1).clamp(max=0)) / 15 if zeros else f.abs().amax(-1) / 7.5
     # half a step inside the range; with a zero point rounded to a level another half at the ends
     assert bool(((back - w).abs().view(40, -1, group) <= (1.01 if zeros else 0.51) * step[..., None] + 1e-6).all())
+
+
+# ----------------------------------------------------------------------------------------------- together, captured, at once
+class Layer:
+    """A decoder layer's attention half: 4-bit products in, append with rotation, attention, 4-bit product out."""
+
+    def __init__(self, gpu, dtype, kv, heads, dim, width, seed):
+        g = _g(seed)
+        self.kv, self.heads, self.dim = kv, heads, dim
+        self.raw = []
+        for n, k in (((heads + 2 * kv) * dim, width), (width, heads * dim)):
+            q = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8)
+            s = ((torch.rand(n, k // 64, generator=g) + 0.5) * (0.25 / math.sqrt(k))).to(dtype)
+            self.raw.append((q, s, None, torch.randn(n, generator=g).to(dtype)))
+        self.w_in, self.w_out = (ops.PackedW4(*(None if t is None else t.to(gpu) for t in r)) for r in self.raw)
+        self.plan = ops.Rotary(dim, device=gpu)
+
+    def __call__(self, x, cache, batch):
+        fused = ops.linear_w4(self.w_in, x).view(x.shape[0], self.heads + 2 * self.kv, self.dim)
+        q, k, v = fused[:, : self.heads], fused[:, self.heads: self.heads + self.kv], fused[:, self.heads + self.kv:]
+        q = ops.kv_append(cache, batch, k, v, rotary=self.plan, q=q)
+        o = ops.paged_attention(q, cache, batch)
+        return fused, q, o, ops.linear_w4(self.w_out, o.view(x.shape[0], -1))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_a_layer_reads_prompts_and_makes_tokens(gpu, dtype):
+    """Ragged prompts in one chunk, then single tokens of all requests: every stage against 64 bits on that stage's own inputs."""
+    kv, heads, dim, width, page = 2, 4, 64, 256, 16
+    layer = Layer(gpu, dtype, kv, heads, dim, width, 3)
+    prompts, steps = [70, 1, 33], 3
+    table = torch.randperm(24, generator=_g(5)).view(3, 8).to(torch.int32)
+    cache = ops.PagedKV.allocate(24, page, kv, dim, dtype, gpu)
+    lens = [0, 0, 0]
+    freq = [10000.0 ** (-2.0 * i / dim) for i in range(dim // 2)]
+    for step in range(1 + steps):
+        new = prompts if step == 0 else [1, 1, 1]
+        before = list(lens)
+        lens = [a + b for a, b in zip(lens, new)]
+        starts = [0, new[0], new[0] + new[1], sum(new)]
+        x = torch.randn(sum(new), width, generator=_g(100 + step)).to(dtype)
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=gpu)  # noqa: E731
+        batch = ops.PagedBatch(table.to(gpu), i32(lens), i32(starts), max(new), max(lens))
+        fused, q, o, y = layer(x.to(gpu), cache, batch)
+        for (w, s, z, b), inp, out in ((layer.raw[0], x, fused.view(sum(new), -1)), (layer.raw[1], o.cpu().view(sum(new), -1), y)):
+            want, mag = O.linear_w4(inp, w, s, z, b)
+            _within(out, want, (u(dtype) + 2 * F) * want.abs() + 8 * 6 * math.sqrt(inp.shape[1]) * F * mag + 2 * F * b.double().abs(), "product")
+        pos = torch.cat([torch.arange(a, b) for a, b in zip(before, lens)])
+        f = fused.cpu()
+        for got, src in ((q, f[:, :heads]), (None, f[:, heads: heads + kv])):
+            want = O.turned(src, pos, freq)
+            if got is None:
+                at = [(int(table[b, p // page]), p % page) for b in range(3) for p in range(before[b], lens[b])]
+                got = torch.stack([cache.k[pg, :, r] for pg, r in at])
+                assert torch.equal(torch.stack([cache.v[pg, :, r] for pg, r in at]).cpu(), f[:, heads + kv:])
+            half = dim // 2
+            size = src.double().abs()
+            pair = torch.cat([size[..., :half] + size[..., half:]] * 2, -1)
+            _within(got, want, u(dtype) * want.abs() * (1 + 8 * F) + pair * 8 * F, "turned")
+        want, mag, reach = O.attend(q.cpu(), cache.k.cpu(), cache.v.cpu(), table.tolist(), lens, starts, dim ** -0.5)
+        rel = 2 * (6 * math.sqrt(dim) + 4) * F * reach + 6 * math.sqrt(max(lens)) * F + (u(dtype) if dtype != torch.float32 else 0.0) + 8 * F
+        _within(o, want, u(dtype) * want.abs() + rel * mag, "attention")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("new,room", [(1, 64), (1, 640), (80, 100)])
+def test_captured_steps_follow_what_is_written_into_the_batch(gpu, dtype, new, room):
+    """A layer captured once and replayed with other lengths, starts and pages, eager work between: each replay the bits of the eager call."""
+    kv, heads, dim, width, page, seqs = 2, 8, 64, 128, 16, 3
+    layer = Layer(gpu, dtype, kv, heads, dim, width, 7)
+    columns = -(-room // page)
+    pages = seqs * columns
+    fixed = dict(table=torch.zeros(seqs, columns, dtype=torch.int32, device=gpu), lens=torch.zeros(seqs, dtype=torch.int32, device=gpu),
+                 starts=torch.zeros(seqs + 1, dtype=torch.int32, device=gpu), x=torch.zeros(seqs * new, width, dtype=dtype, device=gpu))
+    caches = [ops.PagedKV.allocate(pages, page, kv, dim, dtype, gpu) for _ in range(2)]
+    batch = ops.PagedBatch(fixed["table"], fixed["lens"], fixed["starts"], new, room)
+
+    def write(k):
+        g = _g(40 + k)
+        n = [new, max(1, new // (k + 1)), new if k % 2 else 1]
+        start = torch.tensor([0, n[0], n[0] + n[1], sum(n)], dtype=torch.int32)
+        lens = torch.tensor([min(room, n[i] + 7 * k + (room * i) // 3) for i in range(3)], dtype=torch.int32)
+        fixed["table"].copy_(torch.randperm(pages, generator=g).view(seqs, columns).int())
+        fixed["lens"].copy_(lens), fixed["starts"].copy_(start)
+        fixed["x"].copy_(torch.randn(seqs * new, width, generator=g).to(dtype))
+        k0, v0 = (torch.randn(caches[0].k.shape, generator=g).to(dtype) for _ in range(2))
+        for c in caches:
+            c.k.copy_(k0), c.v.copy_(v0)
+        return sum(n)
+
+    write(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(fixed["x"], caches[0], batch)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(fixed["x"], caches[0], batch)
+    for k in range(5):
+        own = write(k)
+        graph.replay()
+        want = layer(fixed["x"], caches[1], batch)
+        torch.cuda.synchronize()
+        for a, b in zip(out[:3], want[:3]):
+            assert torch.equal(a[:own], b[:own]), k
+        assert torch.equal(out[3][:own], want[3][:own]) and torch.equal(caches[0].k, caches[1].k) and torch.equal(caches[0].v, caches[1].v)
+
+
+def test_two_threads_on_two_streams(gpu):
+    """The same plan, cache pages and batch objects used by two threads at once, each on its own stream."""
+    import threading
+
+    c = Case(gpu, torch.bfloat16, [1] * 4, [1500, 900, 1200, 64], 2, 8, 64, 16, seed=11)
+    q = c.q.to(gpu)
+    want = ops.paged_attention(q, c.cache, c.batch)
+    plan = ops.Rotary(64, device=gpu)
+    turned = ops.rotary(plan, q, torch.arange(4, device=gpu))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(50):
+                a, b = ops.paged_attention(q, c.cache, c.batch), ops.rotary(plan, q, torch.arange(4, device=gpu))
+                s.synchronize()
+                if not (torch.equal(a, want) and torch.equal(b, turned)):
+                    bad.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_empty_calls(gpu):
+    """No tokens, no sequences, no rows: nothing is launched, results have their shape."""
+    cache = ops.PagedKV.allocate(2, 4, 1, 8, device=gpu)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=gpu)  # noqa: E731
+    none = ops.PagedBatch(torch.zeros(0, 3, dtype=torch.int32, device=gpu), i32(), i32(0), 0)
+    some = ops.PagedBatch(i32(0, 1).view(1, 2), i32(3), i32(0, 0), 1)
+    flat = ops.PagedBatch(torch.zeros(1, 0, dtype=torch.int32, device=gpu), i32(3), i32(0, 2), 2)
+    x = torch.ones(0, 1, 8, device=gpu)
+    for b in (none, some):
+        assert ops.paged_attention(x, cache, b).shape == (0, 1, 8)
+        ops.kv_append(cache, b, x, x)
+    two = torch.ones(2, 1, 8, device=gpu)
+    ops.kv_append(cache, flat, two, two)                              # a table without columns: no place to write, no key to read
+    assert bool((ops.paged_attention(two, cache, flat) == 0).all()) and bool((cache.k == 0).all())
+    out = torch.full((2, 1, 8), 3.0, device=gpu)
+    assert bool((ops.paged_attention(two, cache, some, out=out) == 3).all())
+    assert ops.rotary(ops.Rotary(8, device=gpu), x, torch.zeros(0, dtype=torch.int64, device=gpu)).shape == (0, 1, 8)
+    pw = ops.PackedW4.quantize(torch.randn(4, 64, device=gpu))
+    assert ops.linear_w4(pw, torch.ones(0, 64, device=gpu)).shape == (0, 4)

@@ -33,9 +33,10 @@ int check_paged_kv(const char *what, const ttsamd_paged_kv *c)
 
 int check_paged_batch(const char *what, const ttsamd_paged_batch *b, int tokens)
 {
-    TTSAMD_CHECK_ARG(b && b->seq_lens && b->q_starts, "%s: the batch is NULL", what);
+    TTSAMD_CHECK_ARG(b, "%s: the batch is NULL", what);
     TTSAMD_CHECK_ARG(b->batch >= 0 && b->batch <= 65535, "%s: batch %d (up to 65535)", what, b->batch);
-    TTSAMD_CHECK_ARG(b->table_width >= 0 && (b->table_width == 0 || b->block_table), "%s: the block table is NULL", what);
+    TTSAMD_CHECK_ARG(b->batch == 0 || (b->seq_lens && b->q_starts), "%s: seq_lens or q_starts is NULL", what);
+    TTSAMD_CHECK_ARG(b->table_width >= 0 && (b->table_width == 0 || b->batch == 0 || b->block_table), "%s: the block table is NULL", what);
     TTSAMD_CHECK_ARG(b->table_stride >= 0 && tokens >= 0 && b->max_new >= 0 && b->max_len >= 0, "%s: negative size", what);
     return TTSAMD_OK;
 }
