@@ -138,8 +138,8 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
     const unsigned flip = g.scale2 < 0.f ? F32 ? 0x80000000u : 0x80008000u : 0u, keep = g.scale2 == 0.f ? 0u : ~0u;
     const float scale2 = g.scale2 == 0.f ? 1.f : fabsf(g.scale2);
 
-    for (int r0 = blockIdx.y * 16 * NQ; r0 < rows; r0 += gridDim.y * 16 * NQ) {
-        const int last = min(r0 + 16 * NQ, rows) - 1;
+    for (int tile = (rows + 16 * NQ - 1) / (16 * NQ) - 1 - blockIdx.y; tile >= 0; tile -= gridDim.y) {      // the longest first
+        const int r0 = tile * 16 * NQ, last = min(r0 + 16 * NQ, rows) - 1;
         Range mine[NQ];
         uint4 q[NQ][NS];
 #pragma unroll
