@@ -215,6 +215,8 @@ ATTEND = [
     ([129, 64, 1, 33, 70], [129, 190, 400, 33, 65], 16, 16, 64, 16), ([40, 90], [40, 350], 16, 64, 128, 64), ([33, 34], [97, 40], 16, 64, 80, 1),
     ([70, 10], [77, 300], 16, 32, 256, 24), ([65, 100], [500, 99], 32, 32, 40, 32), ([128, 128], [256, 129], 16, 32, 200, 8),
     ([129, 1, 70], [129, 400, 65], 2, 8, 64, 16), ([300], [300], 1, 1, 128, 13), ([260, 5], [300, 5], 1, 1, 256, 16),
+    # more of them than the chip holds at once, by one and by two teams of waves
+    ([100, 97, 3], [300, 100, 50], 32, 64, 64, 16), ([130, 70, 5], [130, 200, 40], 64, 64, 64, 24), ([130, 70, 5], [130, 200, 40], 64, 64, 128, 16),
     # the same with the keys split over workgroups
     ([70, 3], [1100, 700], 1, 4, 128, 64), ([300], [900], 1, 1, 256, 24), ([90, 20], [640, 33], 2, 6, 80, 1), ([65, 64], [600, 64], 1, 4, 200, 8),
     ([257], [2000], 1, 1, 64, 16), ([1], [3000], 1, 2, 64, 16), ([9], [2500], 1, 3, 128, 8), ([40], [1500], 1, 1, 256, 32)]

@@ -1,0 +1,26 @@
+// The launches of paged_attention.hip, one translation unit an element type (paged_f32.hip, paged_f16.hip, paged_bf16.hip).
+#pragma once
+#include "paged_stream.h"
+
+namespace ttsamd {
+
+constexpr int kTileKeys = 64, kTile3Keys = 32;      // keys of a staged tile: 16-bit types, fp32
+
+struct PagedLaunch {
+    bool tile;                       // paged_tile.h / paged_tile3.h; else paged_stream.h
+    int dp, nq, waves, teams;        // padded head_dim; row tiles a wave (streamed); waves of a workgroup, or of one of its teams (staged)
+    int splits, split_keys, row_tiles;
+    size_t part_bytes, stat_bytes;
+};
+
+// Waves of a streaming workgroup, by what a wave's registers allow (256 or 512 of them).
+constexpr int most_waves(int dp) { return dp <= 128 ? 8 : 4; }
+
+hipError_t start_f32(const AttArgs &g, const PagedLaunch &p, hipStream_t st);
+hipError_t start_f16(const AttArgs &g, const PagedLaunch &p, hipStream_t st);
+hipError_t start_bf16(const AttArgs &g, const PagedLaunch &p, hipStream_t st);
+void join_f32(const AttArgs &g, hipStream_t st);
+void join_f16(const AttArgs &g, hipStream_t st);
+void join_bf16(const AttArgs &g, hipStream_t st);
+
+}  // namespace ttsamd

@@ -1,6 +1,7 @@
-// Attention of many rows over a paged cache (chunks of a prompt), 16-bit types: keys and values staged through LDS for 128 rows.
+// Attention of many rows over a paged cache (chunks of a prompt), 16-bit types: keys and values staged through LDS for 32 RW rows.
 //
-// A workgroup takes 128 rows (row = token x heads of one key head, as in paged_stream.h), 32 a wave, and walks the keys 64 at a time.
+// A team of RW waves takes 32 rows a wave (row = token x heads of one key head, as in paged_stream.h) and walks the keys 64 at a time;
+// KG teams of a workgroup take the tiles of the same rows in turn and are joined in LDS.
 // As there, S^T = K Q^T is computed, here in 32x32x16 products: a lane holds one row (column lane % 32) and half of a tile's keys, the
 // probabilities are the right operand of O^T = V^T P^T where they lie (slot e of half h of product u is key 16 u + 4 h + e, + 4 for
 // e >= 4), and V^T comes out of LDS by the transposing read, four keys of a channel at a time.
@@ -12,7 +13,7 @@
 //
 // Bound: the matrix unit, with the exponentials (a quarter of the vector rate) next to it.
 #pragma once
-#include "paged_stream.h"
+#include "paged_launch.h"
 
 namespace ttsamd {
 
@@ -31,16 +32,38 @@ template <class T> __device__ __forceinline__ float sum2(unsigned w, float c)
     else return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), h2{(_Float16)1.f, (_Float16)1.f}, c, false);
 }
 
-constexpr int kTileRows = 128, kTileKeys = 64;
-
-template <class T, int DP, bool FULL>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
+// Team 1 hands its running maximum, sum and output to team 0, wave by wave and register by register; all waves of the workgroup call it.
+template <int ND> __device__ __forceinline__ void join_teams(float *lds, int team, int wave, int lane, float &m, float &l, f32x16_t (&o)[ND])
 {
-    constexpr int CH = DP / 8, RB = DP * 2, NSTG = CH / 4, RPI = 64 / CH, NS = DP / 16, ND = DP / 32, AHEAD = 4;
+    float *const mine = lds + wave * (ND * 16 + 2) * 64 + lane;
+    if (team == 1) {
+#pragma unroll
+        for (int x = 0; x < ND; ++x)
+#pragma unroll
+            for (int y = 0; y < 16; ++y) mine[(x * 16 + y) * 64] = o[x][y];
+        mine[ND * 16 * 64] = m, mine[(ND * 16 + 1) * 64] = l;
+    }
+    __syncthreads();
+    if (team == 0) {
+        const float m2 = mine[ND * 16 * 64], to = fmaxf(m, m2), f = __builtin_amdgcn_exp2f(m - to), f2 = __builtin_amdgcn_exp2f(m2 - to);
+        m = to, l = l * f + mine[(ND * 16 + 1) * 64] * f2;
+#pragma unroll
+        for (int x = 0; x < ND; ++x)
+#pragma unroll
+            for (int y = 0; y < 16; ++y) o[x][y] = o[x][y] * f + mine[(x * 16 + y) * 64] * f2;
+    }
+}
+
+template <class T, int DP, bool FULL, int RW, int KG>
+__global__ __launch_bounds__(64 * RW * KG, DP > 128 || (DP == 128 && RW == 2) ? 1 : 2) void attend_tile(AttArgs g)
+{
+    constexpr int CH = DP / 8, RB = DP * 2, NSTG = CH / RW, kTileRows = 32 * RW, RPI = 64 / CH, NS = DP / 16, ND = DP / 32, AHEAD = 4;
     constexpr int HALF = kTileKeys * RB;                    // bytes of a tile's keys (or values)
     extern __shared__ float lds_f[];
     char *const lds = (char *)lds_f;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c32 = lane & 31, h2 = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % RW, c32 = lane & 31, h2 = lane >> 5;
+    const int team = threadIdx.x / (64 * RW);               // KG teams of RW waves take the tiles in turn
+    char *const mem = lds + team * 4 * HALF;
     const int hk = blockIdx.x / g.splits, split = blockIdx.x - hk * g.splits, b = blockIdx.z;
     const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, b);
     const int D = g.c.head_dim, rows = s.n * g.group, tiles = (rows + kTileRows - 1) / kTileRows;
@@ -91,14 +114,14 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
         auto place = [&](int at, int entry) { return at + lane < hi && held(entry, g.c.pages) ? entry : -1; };
         auto stage = [&](const char *src, uint32_t off) {
 #pragma unroll
-            for (int x = 0; x < NSTG; ++x) st[x] = *(const uint4 *)(src + (uint64_t)(uint32_t)__shfl((int)off, (x * 4 + wave) * RPI + row_of_lane) * 16);
+            for (int x = 0; x < NSTG; ++x) st[x] = *(const uint4 *)(src + (uint64_t)(uint32_t)__shfl((int)off, (x * RW + wave) * RPI + row_of_lane) * 16);
         };
         auto k_off = [&](int page, int row) { return page < 0 ? 0 : (uint32_t)page * kpage16 + (uint32_t)row * krow16; };
         auto v_off = [&](int page, int row) { return page < 0 ? 0 : (uint32_t)page * vpage16 + (uint32_t)row * vrow16; };
         auto put_k = [&](char *buf) {
 #pragma unroll
             for (int x = 0; x < NSTG; ++x) {
-                const int r = (x * 4 + wave) * RPI + row_of_lane;
+                const int r = (x * RW + wave) * RPI + row_of_lane;
                 if (!FULL && !piece_in) st[x] = uint4{0, 0, 0, 0};
                 *(uint4 *)(buf + r * RB + ((piece ^ k_swz(r)) & (CH - 1)) * 16) = st[x];
             }
@@ -107,13 +130,13 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
             if (mixed) {
 #pragma unroll
                 for (int x = 0; x < NSTG; ++x) {
-                    if (!(ok >> ((x * 4 + wave) * RPI + row_of_lane) & 1)) st[x] = uint4{0, 0, 0, 0};
+                    if (!(ok >> ((x * RW + wave) * RPI + row_of_lane) & 1)) st[x] = uint4{0, 0, 0, 0};
                     odd |= any_odd<T>(st[x].x) || any_odd<T>(st[x].y) || any_odd<T>(st[x].z) || any_odd<T>(st[x].w);
                 }
             }
 #pragma unroll
             for (int x = 0; x < NSTG; ++x) {
-                const int r = (x * 4 + wave) * RPI + row_of_lane;
+                const int r = (x * RW + wave) * RPI + row_of_lane;
                 if (!FULL && !piece_in) st[x] = uint4{0, 0, 0, 0};
                 *(uint4 *)(buf + HALF + r * RB + ((piece ^ v_swz(r)) & (CH - 1)) * 16) = st[x];
             }
@@ -122,30 +145,33 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
 
         int cur = 0, page_next = -1, row_next = 0;
         uint64_t ok = 0;
+        constexpr int step = KG * kTileKeys;
+        const int begin = lo + team * kTileKeys;
         __syncthreads();                                     // the last row tile's readers are done
-        if (lo < hi) {
+        if (begin < hi) {
             int row;
-            const int page = place(lo, fetch(lo, row));
+            const int page = place(begin, fetch(begin, row));
             ok = __ballot(page >= 0);
-            page_next = fetch(lo + kTileKeys, row_next);
+            page_next = fetch(begin + step, row_next);
             stage(kbase_l, k_off(page, row));
-            put_k(lds);
+            put_k(mem);
             stage(vbase_l, v_off(page, row));
-            put_v(lds, ok, mixed_at(lo, ok));
+            put_v(mem, ok, mixed_at(begin, ok));
         }
-        for (int base = lo; base < hi; base += kTileKeys) {
+        for (int base0 = lo; base0 < hi; base0 += step) {
             __syncthreads();
-            const char *kb = lds + cur * 2 * HALF, *vb = kb + HALF;
-            char *const next = lds + (cur ^ 1) * 2 * HALF;
+            const int base = base0 + team * kTileKeys;
+            const char *kb = mem + cur * 2 * HALF, *vb = kb + HALF;
+            char *const next = mem + (cur ^ 1) * 2 * HALF;
             const uint64_t ok_now = ok;
-            const bool more = base + kTileKeys < hi, busy = base < wlast.end && base + kTileKeys > wfirst.begin;
+            const bool more = base + step < hi, busy = base < hi && base < wlast.end && base + kTileKeys > wfirst.begin;
             uint32_t voff = 0;
             if (more) {
-                const int page = place(base + kTileKeys, page_next);
+                const int page = place(base + step, page_next);
                 ok = __ballot(page >= 0);
                 stage(kbase_l, k_off(page, row_next));
                 voff = v_off(page, row_next);
-                page_next = fetch(base + 2 * kTileKeys, row_next);
+                page_next = fetch(base + 2 * step, row_next);
             }
             f32x16_t sc[2];
             if (busy) {
@@ -226,12 +252,14 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (more) put_v(next, ok, mixed_at(base + kTileKeys, ok));
+            if (more) put_v(next, ok, mixed_at(base + step, ok));
             cur ^= 1;
         }
         const bool redo = __syncthreads_or(odd);
-        if (!redo) {
-            l += __shfl_xor(l, 32);
+        l += __shfl_xor(l, 32);
+        if constexpr (KG == 2)
+            if (!redo) join_teams<ND>(lds_f, team, wave, lane, m, l, o);
+        if (!redo && team == 0) {
             if (r0 + 32 * wave + c32 <= last) {
                 const int64_t token = s.start + my_i, at = (token * g.a.q_heads + my_h) * g.splits + split;
                 const float inv = l > 0.f ? 1.f / l : l;      // no key: zeros; NaN stays
@@ -248,9 +276,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attend_tile(AttArgs g)
                     }
                 if (g.splits > 1 && h2 == 0) g.stat[2 * at] = m, g.stat[2 * at + 1] = l;
             }
-        } else {
-            float *const mine_o = lds_f + wave * 264;
-            for (int r = r0 + wave; r <= last; r += 4) {
+        } else if (redo) {
+            float *const mine_o = lds_f + (team * RW + wave) * 264;
+            for (int r = r0 + team * RW + wave; r <= last; r += RW * KG) {
                 const int i = g.by_group.div(r), h = hk * g.group + r - i * g.group;
                 const int64_t token = s.start + i, at = (token * g.a.q_heads + h) * g.splits + split;
                 Range see = range_of(r);
