@@ -207,7 +207,8 @@ ATTEND = [
     # new, lens, kv_heads, heads, dim, page: single tokens
     ([1], [1], 1, 1, 8, 1), ([1], [2], 1, 1, 64, 16), ([1, 1, 1, 1], [63, 64, 65, 1], 2, 2, 64, 16), ([1, 1], [0, 5], 2, 4, 64, 4),
     ([1, 1], [1000, 777], 2, 6, 128, 64), ([1], [5000], 1, 8, 64, 32), ([1, 1, 0, 1], [129, 31, 40, 256], 1, 16, 80, 24),
-    ([1], [700], 2, 34, 96, 16), ([1, 1], [300, 50], 1, 1, 256, 128), ([1], [513], 3, 3, 40, 7),
+    ([1], [700], 2, 34, 96, 16), ([2, 1, 0], [90, 513, 4], 2, 2, 64, 16), ([1, 1], [33, 700], 2, 4, 128, 5), ([2], [1030], 1, 1, 40, 16),
+    ([1, 1], [2600, 90], 1, 2, 104, 16), ([3, 1], [40, 41], 1, 1, 64, 16), ([1, 1], [300, 50], 1, 1, 256, 128), ([1], [513], 3, 3, 40, 7),
     # chunks
     ([2], [2], 1, 1, 64, 16), ([17, 1, 33], [17, 40, 33], 2, 2, 64, 16), ([5, 64], [100, 64], 1, 3, 128, 1), ([70], [333], 2, 4, 72, 24),
     ([129, 128, 127], [129, 200, 500], 1, 2, 128, 64), ([40], [40], 1, 8, 256, 16), ([300], [310], 2, 2, 32, 13), ([9, 6], [4, 6], 1, 2, 64, 8),

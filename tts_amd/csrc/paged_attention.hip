@@ -23,7 +23,10 @@ PagedLaunch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv 
     // Staged from some rows on (one sequence over 4096 keys; 8 key heads of 128, bf16: 128 / 256 / 1024 rows streamed 28.5 / 30.6 / 57 us,
     // staged 24.6 / 27.2 / 40; 16 of 64, fp32, 2048 keys: 64 / 128 / 256 rows streamed 20.1 / 25.0 / 35, staged 21.5 / 22.9 / 28.6).
     p.tile = f32 ? p.dp <= 128 && rows >= (p.dp == 64 ? 96 : 64) : rows >= 96;
-    p.nq = rows > 16 && p.dp < 256 ? 2 : 1;
+    // One or two fp32 rows go without the matrix unit (one token over 605 keys of 16 heads of 64: 11.4 -> 8.0 us, 48 of up to 1007 keys: 59 ->
+    // 56 us; heads over 128 channels would need more registers than they have).
+    p.few = f32 && rows <= 2 && p.dp <= 128;
+    p.nq = p.few ? (int)rows : rows > 16 && p.dp < 256 ? 2 : 1;
     const bool pairs = p.tile && (p.dp == 64 || (p.dp == 128 && !f32));               // registers and LDS for two teams
     const int kt = p.tile ? f32 ? kTile3Keys : kTileKeys : f32 || p.dp > 128 ? 16 : 32;
     const int64_t key_tiles = keys < 1 ? 1 : (keys + kt - 1) / kt;
@@ -35,7 +38,7 @@ PagedLaunch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv 
         const int64_t small = (rows + 63) / 64 * c.kv_heads * b.batch;
         if (small <= 32 || (small <= kCus && (f32 ? key_tiles <= 16 : p.dp == 64))) p.waves = 2;
     }
-    const int block_rows = p.tile ? 32 * p.waves : 16 * p.nq;
+    const int block_rows = p.tile ? 32 * p.waves : p.few ? p.nq : 16 * p.nq;
     const int64_t tiles = (rows + block_rows - 1) / block_rows, blocks = tiles * c.kv_heads * b.batch;
     p.row_tiles = (int)(tiles < 65535 ? tiles : 65535);
     // Fewer streaming workgroups than compute units: more waves to each, since they are joined in LDS for nothing but a barrier.  (One bf16
@@ -47,13 +50,14 @@ PagedLaunch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv 
     // Still few, and long: the keys are split over workgroups until one round of them fills the chip, and a second launch joins them.
     // (Three tokens over 65537 keys, 12 workgroups of 8 waves, one a compute unit: 21 / 32 / 42 / 85 splits 70.6 / 84.0 / 75.5 / 87.2 us;
     // one bf16 token over 605 keys, 2.4 tiles a wave: whole 8.2 us, two splits 11.0; one over 4096, 16 tiles a wave: at least 1 / 2 / 4
-    // tiles left to a wave 14.1 / 16.0 / 21.0 us.)
+    // tiles left to a wave 14.1 / 16.0 / 21.0 us; one fp32 token over 605, 4.8 tiles a wave: whole 8.0 us, two splits 9.1, over 2048: 17.6
+    // and, eight splits, 12.2.)
     p.splits = 1;
-    const int waves_held = p.tile ? p.dp > 128 || (f32 && p.dp > 64) || (p.waves == 2 && (f32 || p.dp > 64)) ? 4 : 8 : p.dp == 64 ? 12 : p.dp == 128 ? 8 : 4;
+    const int waves_held = p.tile ? p.dp > 128 || (f32 && p.dp > 64) || (p.waves == 2 && (f32 || p.dp > 64)) ? 4 : 8 : p.few ? 16 : p.dp == 64 ? 12 : p.dp == 128 ? 8 : 4;
     const int resident = waves_held / (p.waves * p.teams);                                  // workgroups a compute unit holds, by registers and LDS
     const int64_t fill = (int64_t)kCus * (resident < 1 ? 1 : resident) / blocks, a_wave = p.tile ? p.teams : p.waves;
-    const int64_t most = key_tiles / (a_wave * (p.tile || rows > 64 ? 4 : rows > 32 ? 2 : 1));       // the join costs by the row
-    if (fill > 1 && key_tiles > 4 * a_wave) p.splits = (int)(fill < most ? fill : most);
+    const int64_t most = key_tiles / (a_wave * (p.tile || rows > 64 ? 4 : p.few || rows > 32 ? 2 : 1));       // the join costs by the row
+    if (fill > 1 && key_tiles > (p.few ? 8 : 4) * a_wave) p.splits = (int)(fill < most ? fill : most);
     if ((int64_t)p.splits * c.kv_heads > 65535) p.splits = 65535 / c.kv_heads > 1 ? 65535 / c.kv_heads : 1;
     const int64_t each = (key_tiles + p.splits - 1) / p.splits;
     p.split_keys = (int)(each * kt < 0x7fffffff ? each * kt : 0x7fffffff);

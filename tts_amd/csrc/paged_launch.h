@@ -7,7 +7,7 @@ namespace ttsamd {
 constexpr int kTileKeys = 64, kTile3Keys = 32;      // keys of a staged tile: 16-bit types, fp32
 
 struct PagedLaunch {
-    bool tile;                       // paged_tile.h / paged_tile3.h; else paged_stream.h
+    bool tile, few;                  // paged_tile.h / paged_tile3.h; one or two fp32 rows (attend_few); else attend_stream
     int dp, nq, waves, teams;        // padded head_dim; row tiles a wave (streamed); waves of a workgroup, or of one of its teams (staged)
     int splits, split_keys, row_tiles;
     size_t part_bytes, stat_bytes;

@@ -46,6 +46,20 @@ template <class T, int DP> hipError_t start_tile(const AttArgs &g, const PagedLa
     return start_tile<T, DP, 4, 1>(g, grid, st);
 }
 
+template <int DP, bool FULL, int R> hipError_t start_few(const AttArgs &g, const PagedLaunch &p, dim3 grid, hipStream_t st)
+{
+    static std::atomic<unsigned long long> done{0};
+    const int bytes = p.waves * R * (DP + 4 + 2) * 4, most = most_waves(DP) * R * (DP + 4 + 2) * 4;
+    if (hipError_t e = ensure_dynamic_lds((const void *)attend_few<DP, FULL, R>, most, done)) return e;
+    attend_few<DP, FULL, R><<<grid, p.waves * 64, bytes, st>>>(g);
+    return hipSuccess;
+}
+template <int DP> hipError_t start_few(const AttArgs &g, const PagedLaunch &p, dim3 grid, hipStream_t st)
+{
+    if (g.c.head_dim == DP) return p.nq == 1 ? start_few<DP, true, 1>(g, p, grid, st) : start_few<DP, true, 2>(g, p, grid, st);
+    return p.nq == 1 ? start_few<DP, false, 1>(g, p, grid, st) : start_few<DP, false, 2>(g, p, grid, st);
+}
+
 template <class T> hipError_t start_paged(const AttArgs &g, const PagedLaunch &p, hipStream_t st)
 {
     const dim3 grid(g.c.kv_heads * p.splits, p.row_tiles, g.b.batch);
@@ -54,6 +68,8 @@ template <class T> hipError_t start_paged(const AttArgs &g, const PagedLaunch &p
         if (p.dp == 128) return start_tile<T, 128>(g, p, grid, st);
         if constexpr (sizeof(T) == 2) return start_tile<T, 256>(g, p, grid, st);
     }
+    if constexpr (sizeof(T) == 4)
+        if (p.few) return p.dp == 64 ? start_few<64>(g, p, grid, st) : start_few<128>(g, p, grid, st);
     if (p.dp == 64) return p.nq == 2 ? start_stream<T, 64, 2>(g, p, grid, st) : start_stream<T, 64, 1>(g, p, grid, st);
     if (p.dp == 128) return p.nq == 2 ? start_stream<T, 128, 2>(g, p, grid, st) : start_stream<T, 128, 1>(g, p, grid, st);
     return start_stream<T, 256, 1>(g, p, grid, st);

@@ -68,6 +68,15 @@ template <class T> __device__ __forceinline__ unsigned pack2(float x, float y)
     typedef T t2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f2{x, y}), t2));
 }
+// Both halves of w, added to c in fp32: the probabilities as the products take them, so that what their rounding does to numerator and
+// denominator alike falls out.
+template <class T> __device__ __forceinline__ float sum2(unsigned w, float c)
+{
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), b2{(__bf16)1.f, (__bf16)1.f}, c, false);
+    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), h2{(_Float16)1.f, (_Float16)1.f}, c, false);
+}
 // Whether a 32-bit word of T holds an infinity or NaN.
 template <class T> __device__ __forceinline__ bool any_odd(unsigned w)
 {
@@ -115,6 +124,48 @@ __device__ float attend_row(const AttArgs &g, int b, int hk, const T *q, Range s
         if (lane + 64 * y < D) o[lane + 64 * y] = acc[y];
     if (lane == 0) ml[0] = m, ml[1] = l;
     return l;
+}
+
+// x of the lane N places on in the row of 16.
+template <int N> __device__ __forceinline__ float turned(float x)
+{
+    return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x120 + N, 0xf, 0xf, true));
+}
+
+// Joins the parts o [part][row][DP + 4] and (m, l) [part][row] that lie in LDS and writes the rows r0 .. r0 + nr: to the output, or as one
+// split of it.  R: rows of a part.
+template <class T, int DP>
+__device__ __forceinline__ void join_waves(const AttArgs &g, const Sequence &s, int hk, int split, const float *lds, const float *ml, int r0, int nr,
+                                           int R, int parts)
+{
+    constexpr int LDO = DP + 4;
+    const int D = g.c.head_dim, cols = D / 4;
+    for (int w = threadIdx.x; w < nr * cols; w += blockDim.x) {
+        const int r = w / cols, d = (w - r * cols) * 4;
+        float top = kNoMax, sum = 0.f;
+        f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int x = 0; x < parts; ++x) top = fmaxf(top, ml[2 * (x * R + r)]);
+#pragma unroll 4
+        for (int x = 0; x < parts; ++x) {
+            const float f = __builtin_amdgcn_exp2f(ml[2 * (x * R + r)] - top);
+            sum += f * ml[2 * (x * R + r) + 1];
+            acc += *(const f32x4_t *)(lds + (x * R + r) * LDO + d) * f;
+        }
+        const int row = r0 + r, i = g.by_group.div(row), h = hk * g.group + row - i * g.group;
+        const int64_t token = s.start + i;
+        if (g.splits > 1) {
+            const int64_t at = (token * g.a.q_heads + h) * g.splits + split;
+            *(f32x4_t *)(g.part + at * D + d) = acc;
+            if (d == 0) g.stat[2 * at] = top, g.stat[2 * at + 1] = sum;
+        } else {
+            const float inv = sum > 0.f ? 1.f / sum : sum;          // no key: zeros; NaN stays
+            acc *= inv;
+            T *dst = (T *)g.a.out + token * g.a.o_tstride + (int64_t)h * g.a.o_hstride + d;
+            if constexpr (sizeof(T) == 4) *(f32x4_t *)dst = acc;
+            else *(uint2 *)dst = uint2{pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3])};
+        }
+    }
 }
 
 template <class T, int DP, int NQ, bool FULL, int MAXW>
@@ -279,7 +330,7 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
 #pragma unroll
                 for (int e = 0; e < VK; ++e) {
                     p[u][e] = __builtin_amdgcn_exp2f(fmaf(sc[u][e >> 2][e & 3], scale2, -m[u]));
-                    l[u] += p[u][e];
+                    if constexpr (F32) l[u] += p[u][e];
                 }
             }
             if constexpr (F32) {
@@ -293,7 +344,10 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
             } else if constexpr (KT == 16) {
                 uint2 pb[NQ];
 #pragma unroll
-                for (int u = 0; u < NQ; ++u) pb[u] = uint2{pack2<T>(p[u][0], p[u][1]), pack2<T>(p[u][2], p[u][3])};
+                for (int u = 0; u < NQ; ++u) {
+                    pb[u] = uint2{pack2<T>(p[u][0], p[u][1]), pack2<T>(p[u][2], p[u][3])};
+                    l[u] = sum2<T>(pb[u].x, sum2<T>(pb[u].y, l[u]));
+                }
 #pragma unroll
                 for (int x = 0; x < NV; ++x) {
                     const unsigned sel = x & 1 ? 0x07060302u : 0x05040100u;
@@ -304,8 +358,10 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
             } else {
                 uint4 pb[NQ];
 #pragma unroll
-                for (int u = 0; u < NQ; ++u)
+                for (int u = 0; u < NQ; ++u) {
                     pb[u] = uint4{pack2<T>(p[u][0], p[u][1]), pack2<T>(p[u][2], p[u][3]), pack2<T>(p[u][4], p[u][5]), pack2<T>(p[u][6], p[u][7])};
+                    l[u] = sum2<T>(pb[u].x, sum2<T>(pb[u].y, sum2<T>(pb[u].z, sum2<T>(pb[u].w, l[u]))));
+                }
 #pragma unroll
                 for (int x = 0; x < NV; ++x) {
                     const unsigned sel = x & 1 ? 0x07060302u : 0x05040100u;
@@ -345,33 +401,154 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
             }
         }
         __syncthreads();
-        const int cols = D / 4, nr = last - r0 + 1, parts = redo ? 1 : waves;
-        for (int w = threadIdx.x; w < nr * cols; w += blockDim.x) {
-            const int r = w / cols, d = (w - r * cols) * 4;
-            float top = kNoMax, sum = 0.f;
-            f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-            for (int x = 0; x < parts; ++x) top = fmaxf(top, ml[2 * (x * R + r)]);
-#pragma unroll 4
-            for (int x = 0; x < parts; ++x) {
-                const float f = __builtin_amdgcn_exp2f(ml[2 * (x * R + r)] - top);
-                sum += f * ml[2 * (x * R + r) + 1];
-                acc += *(const f32x4_t *)(lds + (x * R + r) * LDO + d) * f;
-            }
-            const int row = r0 + r, i = g.by_group.div(row), h = hk * g.group + row - i * g.group;
-            const int64_t token = s.start + i;
-            if (g.splits > 1) {
-                const int64_t at = (token * g.a.q_heads + h) * g.splits + split;
-                *(f32x4_t *)(g.part + at * D + d) = acc;
-                if (d == 0) g.stat[2 * at] = top, g.stat[2 * at + 1] = sum;
-            } else {
-                const float inv = sum > 0.f ? 1.f / sum : sum;          // no key: zeros; NaN stays
-                acc *= inv;
-                T *dst = (T *)g.a.out + token * g.a.o_tstride + (int64_t)h * g.a.o_hstride + d;
-                if constexpr (F32) *(f32x4_t *)dst = acc;
-                else *(uint2 *)dst = uint2{pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3])};
+        join_waves<T, DP>(g, s, hk, split, lds, ml, r0, last - r0 + 1, R, redo ? 1 : waves);
+    }
+}
+
+// One or two fp32 rows: the same stream without the matrix unit, whose fp32 products of 16 rows would leave 14 of them idle at 1152 cycles
+// a tile of 16 keys of 64 channels, against some 360 here.  A lane holds four channels of every 64 of keys 4 (lane / 16) + i: whole rows
+// of 16 lanes add up a score by rotation, so that the lanes of a key know it, and each 16 lanes keep a maximum, sum and output of their
+// own until the end.
+template <int DP, bool FULL, int R> __global__ __launch_bounds__(512) void attend_few(AttArgs g)
+{
+    constexpr int NX = DP / 64, KT = 16;
+    extern __shared__ float lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int c16 = lane & 15, g4 = lane >> 4;
+    const int hk = blockIdx.x / g.splits, split = blockIdx.x - hk * g.splits, b = blockIdx.z;
+    const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, b);
+    const int D = g.c.head_dim, rows = s.n * g.group;
+    const char *kbase = (const char *)g.c.k + (int64_t)hk * g.c.k_head * 4, *vbase = (const char *)g.c.v + (int64_t)hk * g.c.v_head * 4;
+    const bool vrole = lane >= 32;
+    const uint32_t page16 = (uint32_t)((vrole ? g.c.v_page : g.c.k_page) / 4), row16 = (uint32_t)((vrole ? g.c.v_row : g.c.k_row) / 4);
+    const float flip = g.scale2 < 0.f ? -1.f : g.scale2 == 0.f ? 0.f : 1.f, scale2 = g.scale2 == 0.f ? 1.f : fabsf(g.scale2);
+    for (int r0 = blockIdx.y * R; r0 < rows; r0 += gridDim.y * R) {
+        const int last = min(r0 + R, rows) - 1;
+        Range mine[R], all = {0x7fffffff, 0};
+        f32x4_t q[R][NX];
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const int r = min(r0 + u, last), i = g.by_group.div(r), h = hk * g.group + r - i * g.group;
+            mine[u] = seen_by(s, s.len - s.n + i, g.a.causal, g.a.window);
+            all.begin = min(all.begin, mine[u].begin), all.end = max(all.end, mine[u].end);
+            const float *src = (const float *)g.a.q + (int64_t)(s.start + i) * g.a.q_tstride + (int64_t)h * g.a.q_hstride;
+#pragma unroll
+            for (int x = 0; x < NX; ++x) {
+                const int d = c16 * 4 + 64 * x;
+                q[u][x] = FULL || d < D ? *(const f32x4_t *)(src + (FULL || d < D ? d : 0)) * flip : f32x4_t{0.f, 0.f, 0.f, 0.f};
             }
         }
+        const int64_t from = all.begin + (int64_t)split * g.split_keys, to = split + 1 < g.splits ? from + g.split_keys : all.end;
+        const int lo = (int)min(from, (int64_t)all.end), hi = (int)min(to, (int64_t)all.end);
+        f32x4_t o[R][NX], k[4][NX], v[4][NX];
+        float m[R], l[R];
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            m[u] = kNoMax, l[u] = 0.f;
+#pragma unroll
+            for (int x = 0; x < NX; ++x) o[u][x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+        const int step = waves * KT;
+        int base = lo + wave * KT;
+        auto fetch = [&](int at, int &row) { return entry_of(g.b, g.by_page, b, min(at + c16, hi - 1), row); };
+        auto place = [&](int at, int entry) { return at + c16 < hi && held(entry, g.c.pages) ? entry : -1; };
+        // keys in lanes 0-15, values in 32-47: where the four of this lane's sixteen lie
+        auto load = [&](f32x4_t(&to)[4][NX], const char *from, uint32_t off, int role) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const char *p = from + (uint64_t)(uint32_t)__shfl((int)off, role + 4 * g4 + i) * 16;
+#pragma unroll
+                for (int x = 0; x < NX; ++x) {
+                    const int d = c16 * 4 + 64 * x;
+                    to[i][x] = *(const f32x4_t *)(p + (FULL || d < D ? d * 4 : 0));
+                    if (!FULL && d >= D) to[i][x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                }
+            }
+        };
+        int row_next = 0, entry_next = -1;
+        uint32_t off = 0;
+        unsigned ok = 0;
+        if (base < hi) {
+            int row;
+            const int page = place(base, fetch(base, row));
+            off = page < 0 ? 0 : (uint32_t)page * page16 + (uint32_t)row * row16;
+            ok = (unsigned)__ballot(page >= 0) & 0xffffu;
+            load(k, kbase, off, 0);
+            entry_next = fetch(base + step, row_next);
+        }
+        for (; base < hi; base += step) {
+            load(v, vbase, off, 32);
+            const unsigned ok_now = ok;
+            const int page = place(base + step, entry_next);
+            off = page < 0 ? 0 : (uint32_t)page * page16 + (uint32_t)row_next * row16;
+            ok = (unsigned)__ballot(page >= 0) & 0xffffu;
+            entry_next = fetch(base + 2 * step, row_next);
+            float sc[R][4];
+#pragma unroll
+            for (int u = 0; u < R; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float x = 0.f;
+#pragma unroll
+                    for (int y = 0; y < NX; ++y)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x = fmaf(q[u][y][e], k[i][y][e], x);
+                    x += turned<8>(x), x += turned<4>(x), x += turned<2>(x), x += turned<1>(x);
+                    sc[u][i] = x;
+                }
+            if (base + step < hi) load(k, kbase, off, 0);
+#pragma unroll
+            for (int u = 0; u < R; ++u) {
+                const uint32_t bits = (uint32_t)seen_bits(ok_now, base, mine[u]) >> (4 * g4);
+                float top = kNoMax;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sc[u][i] = masked(sc[u][i], bits, i);
+                    top = fmaxf(top, sc[u][i] * scale2);
+                }
+                if (__any(top > m[u] + kLazy)) {
+                    const float to = fmaxf(m[u], top), fade = __builtin_amdgcn_exp2f(m[u] - to);
+                    m[u] = to, l[u] *= fade;
+#pragma unroll
+                    for (int x = 0; x < NX; ++x) o[u][x] *= fade;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][i], scale2, -m[u]));
+                    l[u] += p;
+#pragma unroll
+                    for (int x = 0; x < NX; ++x)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            // a key that is not seen takes no part, whatever its value holds
+                            const float value = bits >> i & 1 ? v[i][x][e] : 0.f;
+                            o[u][x][e] = fmaf(p, value, o[u][x][e]);
+                        }
+                }
+            }
+        }
+        // join the 16 lanes' results of a wave, then the waves
+        constexpr int LDO = DP + 4;
+        float *const ml = lds + waves * R * LDO;
+        __syncthreads();                                    // the last rows' readers are done
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            float top = fmaxf(m[u], __shfl_xor(m[u], 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float f = __builtin_amdgcn_exp2f(m[u] - top);
+            float sum = l[u] * f;
+            sum += __shfl_xor(sum, 16), sum += __shfl_xor(sum, 32);
+#pragma unroll
+            for (int x = 0; x < NX; ++x) {
+                f32x4_t y = o[u][x] * f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], 16), y[e] += __shfl_xor(y[e], 32);
+                if (g4 == 0) *(f32x4_t *)(lds + (wave * R + u) * LDO + c16 * 4 + 64 * x) = y;
+            }
+            if (lane == 0) ml[2 * (wave * R + u)] = top, ml[2 * (wave * R + u) + 1] = sum;
+        }
+        __syncthreads();
+        join_waves<float, DP>(g, s, hk, split, lds, ml, r0, last - r0 + 1, R, waves);
     }
 }
 

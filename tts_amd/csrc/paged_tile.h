@@ -23,15 +23,6 @@ template <class T> __device__ __forceinline__ f32x16_t mfma_32x32x16(uint4 a, ui
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-// Both halves of w, added to c in fp32.
-template <class T> __device__ __forceinline__ float sum2(unsigned w, float c)
-{
-    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), b2{(__bf16)1.f, (__bf16)1.f}, c, false);
-    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), h2{(_Float16)1.f, (_Float16)1.f}, c, false);
-}
-
 // Team 1 hands its running maximum, sum and output to team 0, wave by wave and register by register; all waves of the workgroup call it.
 template <int ND> __device__ __forceinline__ void join_teams(float *lds, int team, int wave, int lane, float &m, float &l, f32x16_t (&o)[ND])
 {
