@@ -720,7 +720,8 @@ typedef struct ttsamd_paged_batch {
 
 /* Writes the new tokens' keys and values into the cache, the keys (and the queries, if given) rotated on the way, as one launch.
  * plan NULL: nothing rotates.  positions NULL: a token turns by its place in the cache; else by positions[token].
- * Element type of every tensor = the cache's.  No two tokens of a call may share a place of the cache. */
+ * Element type of every tensor = the cache's.  No two tokens of a call may share a place of the cache.  Rows of q_out behind the last
+ * sequence are left as they were. */
 typedef struct ttsamd_kv_append_args {
     const void *k, *v;                    /* [tokens, kv_heads, head_dim] */
     int64_t k_tstride, k_hstride, v_tstride, v_hstride;
@@ -737,8 +738,8 @@ int ttsamd_kv_append(const ttsamd_kv_append_args *args /* host */, const ttsamd_
  * hold a key, with j <= p when causal != 0 and j > p - window when window > 0; p = t's position.  Query head h reads key head
  * h / (q_heads / kv_heads).  A row that sees no key is zero.  Rows of `out` behind the last sequence are left as they were.
  * Statistics and sums in fp32.  head_dim a multiple of 8 up to 256; q, out and the cache start and stride at 16 bytes.
- * `workspace` (device, ttsamd_paged_attention_workspace_bytes; 16-byte aligned; nothing is kept in it between calls): partial
- * results where a long cache is split over the chip. */
+ * `workspace` (device, ttsamd_paged_attention_workspace_bytes, at most 256 MiB; 16-byte aligned; nothing is kept in it between calls, and
+ * no two calls that may run at once share one): partial results where a long cache is split over the chip. */
 typedef struct ttsamd_paged_attention_args {
     const void *q;                        /* [tokens, q_heads, head_dim] */
     void *out;

@@ -333,6 +333,21 @@ def test_paged_attention_positions_beyond_32_bits_of_bytes(gpu):
     assert torch.equal(cache.k[int(c.table[0, 6]), :, 3], new_k[0])
 
 
+@pytest.mark.parametrize("trailing", [0, 500, 9000])
+def test_paged_attention_workspace_stays_small_when_tokens_are_padding(gpu, trailing):
+    """A long cache read by one token of a call sized for thousands: few or no parts, the same result."""
+    import ctypes
+
+    c = Case(gpu, torch.bfloat16, [1, 1], [4000, 3500], 2, 16, 64, 16, seed=13, trailing=trailing)
+    a = ops._PagedAttentionArgs(tokens=c.tokens, q_heads=16, causal=1, scale=1.0)
+    need = _lib.lib().ttsamd_paged_attention_workspace_bytes(bytes(a), ctypes.c_void_p(c.cache._ref), ctypes.c_void_p(c.batch._ref))
+    assert need <= 256 << 20 and (trailing > 0 or need > 0)
+    out = torch.full(c.q.shape, 2.0, dtype=c.dtype, device=gpu)
+    ops.paged_attention(c.q.to(gpu), c.cache, c.batch, out=out)
+    assert bool((out[2:] == 2).all())
+    c.check(out, what="padded")
+
+
 # ------------------------------------------------------------------------------------------------------------------- w4
 def _w4(dtype, m, n, k, group, zeros, bias, seed):
     g = _g(seed)

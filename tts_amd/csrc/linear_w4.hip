@@ -181,8 +181,9 @@ template <class T, int NT, int GROUP> hipError_t start(const ttsamd_linear_w4_ar
 {
     constexpr int MAXW = NT == 1 && sizeof(T) == 2 ? 16 : 8;
     const int chunks = (a.k + 127) / 128, blocks = (a.n + 16 * NT - 1) / (16 * NT), row_blocks = (a.m + 15) / 16;
+    const bool few = (int64_t)blocks * row_blocks < 256;
     // Waves share the chunks of k: eight, or sixteen where there are fewer workgroups than compute units.
-    int waves = MAXW > 8 && blocks * row_blocks < 256 ? 16 : 8;
+    int waves = MAXW > 8 && few ? 16 : 8;
     while (waves > 1 && waves > chunks) waves /= 2;
     const int rows = a.m < 16 ? a.m : 16, bytes = waves * rows * (16 * NT + 1) * 4;
     static std::atomic<unsigned long long> done{0};
@@ -224,8 +225,8 @@ extern "C" int ttsamd_linear_w4(const ttsamd_linear_w4_args *a, void *stream)
     TTSAMD_CHECK_ARG(a->x && a->y && a->levels && a->scales, "linear_w4: a tensor is NULL");
     TTSAMD_CHECK_ARG((((uintptr_t)a->levels | (uintptr_t)a->scales | (uintptr_t)a->zeros) & 15) == 0,
                      "linear_w4: levels, scales and zeros start at multiples of 16 bytes");
-    if (a->m > 65535 * 16) {
-        set_error("linear_w4: %d rows (up to 2^20 - 16)", a->m);
+    if (a->m > 65535 * 16 || a->n > (1 << 30) || a->k > (1 << 30)) {
+        set_error("linear_w4: %d rows, %d by %d weights (up to 2^20 - 16 rows, 2^30 a side)", a->m, a->n, a->k);
         return TTSAMD_ERR_UNSUPPORTED;
     }
     hipStream_t st = as_stream(stream);

@@ -58,6 +58,9 @@ PagedLaunch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv 
     const int64_t fill = (int64_t)kCus * (resident < 1 ? 1 : resident) / blocks, a_wave = p.tile ? p.teams : p.waves;
     const int64_t most = key_tiles / (a_wave * (p.tile || rows > 64 ? 4 : p.few || rows > 32 ? 2 : 1));       // the join costs by the row
     if (fill > 1 && key_tiles > (p.few ? 8 : 4) * a_wave) p.splits = (int)(fill < most ? fill : most);
+    // Parts are laid out by the token, whoever owns it: a call whose tokens are mostly padding gets fewer splits, not gigabytes.
+    const size_t rows_bytes = (size_t)a.tokens * a.q_heads * (c.head_dim + 2) * sizeof(float), room_bytes = (size_t)256 << 20;
+    if (p.splits * rows_bytes > room_bytes) p.splits = rows_bytes * 2 > room_bytes ? 1 : (int)(room_bytes / rows_bytes);
     if ((int64_t)p.splits * c.kv_heads > 65535) p.splits = 65535 / c.kv_heads > 1 ? 65535 / c.kv_heads : 1;
     const int64_t each = (key_tiles + p.splits - 1) / p.splits;
     p.split_keys = (int)(each * kt < 0x7fffffff ? each * kt : 0x7fffffff);

@@ -1055,7 +1055,8 @@ def _same_device(batch, cache):
 def kv_append(cache, batch, k, v, rotary=None, q=None, positions=None, q_out=None):
     """Writes k, v [tokens, kv_heads, head_dim] of the batch's new tokens to their places in the cache; with a `rotary` plan the keys, and
     q [tokens, q_heads, head_dim] if given, turn on the way.  Returns the turned q (in `q_out`, which may be q; default: a new tensor), or
-    None.  Tokens turn by their place in the cache, or by `positions` [tokens].  One launch."""
+    None.  Tokens turn by their place in the cache, or by `positions` [tokens].  Rows of `q_out` behind the last sequence are left as they
+    were.  One launch."""
     tokens, dtype, device = k.shape[0], cache.dtype, cache.device
     shape = (tokens, cache.kv_heads, cache.head_dim)
     kt, kh = _rows(k, "k", shape, dtype, device)
@@ -1145,18 +1146,22 @@ class PackedW4:
         _need(all(t is None or t.device == qweight.device for t in (scales, zeros, bias)), "qweight, scales, zeros and bias are on one device")
         tiles, chunks = -(-n // 16), -(-k // 128)
         per = 128 // group
-        full = torch.zeros((tiles * 16, chunks * 64), dtype=torch.uint8, device=qweight.device)
-        full[:n, : k // 2] = qweight
+
+        def padded(t, columns):
+            if t.shape == (tiles * 16, columns):
+                return t.contiguous()
+            f = torch.zeros((tiles * 16, columns), dtype=t.dtype, device=t.device)
+            f[: t.shape[0], : t.shape[1]] = t
+            return f
+
         # of eight levels 0 .. 7 in four bytes, the even ones go to the lower half of the word, the odd ones to the upper
-        b = full.view(-1, 2, 2)
-        full = torch.stack([b[..., 0] & 15 | b[..., 1] << 4, b[..., 0] >> 4 | b[..., 1] & 240], 1).contiguous()
-        words = full.view(-1).view(torch.int32).view(tiles, 16, chunks, 4, 4)                     # [t, r, c, j, g]
+        b = padded(qweight, chunks * 64).view(-1, 2, 2)
+        halves = torch.stack([b[..., 0] & 15 | b[..., 1] << 4, b[..., 0] >> 4 | b[..., 1] & 240], 1)
+        words = halves.view(-1).view(torch.int32).view(tiles, 16, chunks, 4, 4)          # [t, r, c, j, g]
         self.levels = words.permute(0, 2, 4, 1, 3).contiguous()                          # [t, c, g, r, j]
 
         def by_group(t):
-            f = torch.zeros((tiles * 16, chunks * per), dtype=t.dtype, device=t.device)
-            f[:n, : k // group] = t
-            return f.view(tiles, 16, chunks * per).transpose(1, 2).contiguous()
+            return padded(t, chunks * per).view(tiles, 16, chunks * per).transpose(1, 2).contiguous()
 
         self.scales = by_group(scales)
         self.zeros = None if zeros is None else by_group(zeros)
