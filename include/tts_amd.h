@@ -753,7 +753,7 @@ int ttsamd_paged_attention(const ttsamd_paged_attention_args *args /* host */, c
                            const ttsamd_paged_batch *batch /* host */, void *workspace, size_t workspace_bytes, void *stream);
 
 /* y[m, n] = sum_k x[m, k] * (level[n, k] - zero[n, k / group]) * scale[n, k / group] + bias[n]: a layer with 4-bit weights for the few
- * rows of a decoding step.  Levels 0..15; without zero points the zero is 8.  fp32 sums of exact products.
+ * rows of a decoding step.  Levels and zeros 0..15; without zero points the zero is 8.  fp32 sums of exact products.
  * `levels`: the image [ceil(n/16)][ceil(k/128)][4 g][16 r][4 j] of 32-bit words; word (g, r, j) of tile (t, c) holds the levels of
  * output 16 t + r at k = 128 c + 32 j + 8 g + e, e = 0..7: level 2p from bit 4p, level 2p + 1 from bit 16 + 4p.  `scales` / `zeros`: [ceil(n/16)][groups of the
  * padded k][16 r], scales in scale_dtype, zeros uint8 (or NULL); padding has scale 0.  All three start at 16 bytes. */

@@ -123,6 +123,8 @@ def _refused(fn, want, *args):
 
 def test_c_refusals_come_before_any_launch():
     """The C entries check what the kernels assume; the pointers here are never followed."""
+    for what, arguments in (("rotary", 1), ("kv_append", 3), ("paged_attention", 4), ("linear_w4", 0)):
+        ops._entry(what, arguments)                                         # what the Python views call leaves the library's own attribute alone
     ref, P = ctypes.byref, 4096
     plan = ops._RotaryPlan(P, 64, 0, 1.0)
     good = dict(x=P, y=P, x_tstride=64, x_hstride=64, y_tstride=64, y_hstride=64, positions=P, position_bytes=8, tokens=1, heads=1, head_dim=64, dtype=0)

@@ -395,6 +395,26 @@ def test_linear_w4_scales_of_any_type_and_non_finite_rows(gpu, scale_dtype):
     assert bool(torch.isnan(got[1]).all()) and not bool(torch.isfinite(got[2]).any())
 
 
+@pytest.mark.parametrize("dtype,m,n,k,group", [(torch.float32, 5, 50, 384, 128), (torch.float16, 17, 33, 256, 64), (torch.bfloat16, 3, 16, 96, 32)])
+def test_linear_w4_infinities_and_the_largest_values(gpu, dtype, m, n, k, group):
+    """An infinity takes every output to the infinity (or NaN, at a weight of zero) that the plain sum gives; a finite sum of the type's
+    largest values stays finite."""
+    x, q, s, z, _ = _w4(dtype, m, n, k, group, True, False, 4)
+    s = s.sign() * 2.0 ** -8
+    x[0, k // 3], x[1, 5], x[1, k - 1], x[2, 0] = math.inf, -math.inf, -math.inf, torch.finfo(dtype).max
+    level = torch.stack([q & 15, q >> 4], -1).view(n, k).double()
+    w = (level - z.repeat_interleave(group, 1).double()) * s.repeat_interleave(group, 1).double()
+    want = (x.double()[:, None] * w).sum(-1)
+    assert not bool(torch.isfinite(want[:2]).any()) and bool(torch.isfinite(want[2:]).all())
+    got = ops.linear_w4(ops.PackedW4(q.to(gpu), s.to(gpu), z.to(gpu)), x.to(gpu)).cpu().double()
+    assert torch.equal(torch.isnan(got[:2]), torch.isnan(want[:2]))
+    same = ~torch.isnan(want[:2])
+    assert torch.equal(got[:2][same], want[:2][same])
+    # k roundings of sums no larger than the sum of the products' sizes (six times it where x (16 + q) meets x (16 + z)), one to the type
+    mag = (x.double()[2:, None] * w).abs().sum(-1)
+    assert bool(((got[2:] - want[2:]).abs() <= 6 * k * F * mag + torch.finfo(dtype).eps / 2 * want[2:].abs()).all())
+
+
 @pytest.mark.parametrize("zeros", [False, True])
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_quantize_is_within_half_a_step(gpu, group, zeros):

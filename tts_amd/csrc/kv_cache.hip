@@ -101,11 +101,12 @@ template <class T, int V> __global__ __launch_bounds__(256) void move_rows(MoveA
     }
     const int half = a.plan.rotary_dim / 2;
     using P = Piece<T, V>;
-    for (int t0 = blockIdx.x * a.token_tile; t0 < n; t0 += gridDim.x * a.token_tile) {
-        const int items = min(a.token_tile, n - t0) * a.units;
+    // unsigned: the step past the last token of 2^31 is no negative one
+    for (unsigned t0 = blockIdx.x * a.token_tile; t0 < (unsigned)n; t0 += gridDim.x * a.token_tile) {
+        const int items = min(a.token_tile, n - (int)t0) * a.units;
         for (int w = threadIdx.x; w < items; w += 256) {
             const int lt = a.by_units.div(w), unit = w - lt * a.units;
-            const int i = t0 + lt, token = start + i;
+            const int i = (int)t0 + lt, token = start + i;
             const int which = unit >= a.s[2].first_unit ? 2 : unit >= a.s[1].first_unit ? 1 : 0;
             const Stream &st = a.s[which];
             const int turning = st.turns ? half / V : 0;

@@ -40,6 +40,29 @@ template <bool BF> __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4
 // The upper halves of x and y.
 __device__ __forceinline__ unsigned uppers(unsigned x, unsigned y) { return __builtin_amdgcn_perm(y, x, 0x07060302u); }
 
+// Output n of row m product by product, for a sum that is no number: an infinity takes x (16 + q) and x (16 + z) apart into NaN, and fp32
+// values from 2^123 on can pass fp32's range there, where x times the weight need not.
+template <class T, int GROUP> __device__ float summed(const ttsamd_linear_w4_args &a, int m, int n)
+{
+    const T *x = (const T *)a.x + (int64_t)m * a.x_stride;
+    const int chunks = (a.k + 127) / 128;
+    const int64_t tile = n / 16;
+    const unsigned *words = a.levels + (tile * chunks * 64 + n % 16) * 4;
+    float y = a.bias ? to_f(((const T *)a.bias)[n]) : 0.f;
+    for (int q = 0; q < a.k / GROUP; ++q) {
+        const int64_t at = (tile * chunks * (128 / GROUP) + q) * 16 + n % 16;
+        const float z = a.zeros ? (float)a.zeros[at] : 8.f;
+        const float scale = a.scale_dtype == TTSAMD_F32    ? ((const float *)a.scales)[at]
+                            : a.scale_dtype == TTSAMD_BF16 ? (float)((const __bf16 *)a.scales)[at]
+                                                           : (float)((const _Float16 *)a.scales)[at];
+        for (int k = q * GROUP; k < (q + 1) * GROUP; ++k) {
+            const unsigned w = words[((int64_t)(k / 128) * 64 + (k / 8 % 4) * 16) * 4 + k / 32 % 4];
+            y = fmaf(to_f(x[k]), ((float)(w >> (4 * (k / 2 % 4) + 16 * (k % 2)) & 15) - z) * scale, y);
+        }
+    }
+    return y;
+}
+
 template <class T, int NT, int GROUP, int MAXW> __global__ __launch_bounds__(MAXW * 64) void linear_w4(ttsamd_linear_w4_args a)
 {
     constexpr bool F32 = sizeof(T) == 4, BF = !__is_same(T, _Float16);
@@ -47,7 +70,7 @@ template <class T, int NT, int GROUP, int MAXW> __global__ __launch_bounds__(MAX
     constexpr int RAW = F32 ? 2 : 1;                                             // 16-byte pieces of eight k of x
     constexpr bool XAHEAD = !F32 && NT < 4;
     extern __shared__ float join[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int chunks = (a.k + 127) / 128, m0 = blockIdx.y * 16, rows = min(a.m - m0, 16);
     const int c16 = lane & 15, g4 = lane >> 4, row = 4 * (c16 & 3) + (c16 >> 2);
     unsigned one = BF ? 0x41804180u : 0x4c004c00u;
@@ -173,6 +196,7 @@ template <class T, int NT, int GROUP, int MAXW> __global__ __launch_bounds__(MAX
         float y = a.bias ? to_f(((const T *)a.bias)[n]) : 0.f;
 #pragma unroll 4
         for (int x = 0; x < waves; ++x) y += join[(x * rows + r) * LD + col];
+        if (!(fabsf(y) < __builtin_inff())) y = summed<T, GROUP>(a, m0 + r, n);
         ((T *)a.y)[(int64_t)(m0 + r) * a.y_stride + n] = (T)y;
     }
 }

@@ -176,7 +176,7 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
     constexpr int VK = KT / 4;                          // values (keys) a lane holds of a tile
     constexpr int VB = NV * ES, VP = VB < 16 ? 8 : 16;  // bytes of a lane's channels of one key, and of one load
     extern __shared__ float lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int c16 = lane & 15, g4 = lane >> 4;
     const int hk = blockIdx.x / g.splits, split = blockIdx.x - hk * g.splits, b = blockIdx.z;
     const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, b);
@@ -413,7 +413,7 @@ template <int DP, bool FULL, int R> __global__ __launch_bounds__(512) void atten
 {
     constexpr int NX = DP / 64, KT = 16;
     extern __shared__ float lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int c16 = lane & 15, g4 = lane >> 4;
     const int hk = blockIdx.x / g.splits, split = blockIdx.x - hk * g.splits, b = blockIdx.z;
     const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, b);

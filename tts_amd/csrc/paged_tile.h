@@ -52,8 +52,8 @@ __global__ __launch_bounds__(64 * RW * KG, DP > 128 || (DP == 128 && RW == 2) ? 
     constexpr int HALF = kTileKeys * RB;                    // bytes of a tile's keys (or values)
     extern __shared__ float lds_f[];
     char *const lds = (char *)lds_f;
-    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % RW, c32 = lane & 31, h2 = lane >> 5;
-    const int team = threadIdx.x / (64 * RW);               // KG teams of RW waves take the tiles in turn
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % RW), c32 = lane & 31, h2 = lane >> 5;
+    const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * RW));               // KG teams of RW waves take the tiles in turn
     char *const mem = lds + team * 4 * HALF;
     const int hk = blockIdx.x / g.splits, split = blockIdx.x - hk * g.splits, b = blockIdx.z;
     const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, b);

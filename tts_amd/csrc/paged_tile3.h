@@ -55,8 +55,8 @@ template <int DP, bool FULL, int RW, int KG> __global__ __launch_bounds__(64 * R
     constexpr int CH = DP / 8, RB = DP * 2, PLANE = kTile3Keys * RB, NST = kTile3Keys * CH / (64 * RW), kTileRows = 32 * RW, NS = DP / 16, ND = DP / 32;
     extern __shared__ float lds_f[];
     char *const lds = (char *)lds_f;
-    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % RW, c32 = lane & 31, h2 = lane >> 5;
-    const int team = threadIdx.x / (64 * RW), member = threadIdx.x % (64 * RW);       // KG teams of RW waves take the tiles in turn
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % RW), c32 = lane & 31, h2 = lane >> 5;
+    const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * RW)), member = threadIdx.x % (64 * RW);       // KG teams of RW waves take the tiles in turn
     char *const mem = lds + team * 12 * PLANE;
     const int hk = blockIdx.x / g.splits, split = blockIdx.x - hk * g.splits, b = blockIdx.z;
     const Sequence s = sequence_of(g.b, g.a.tokens, g.c.page_size, b);

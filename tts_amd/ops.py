@@ -780,7 +780,7 @@ def sample_gaussian(stats, noise, mask):
 # Autoregressive decoding (include/tts_amd.h, last section): rotary positions, a paged key/value cache, attention over it and
 # products with 4-bit weights.  Token-major [tokens, heads, head_dim] tensors in float32, float16 or bfloat16.  Work is queued on
 # the tensors' device, on its current stream.  All of it can be captured into a graph: nothing waits for the device, and sizes
-# that vary from step to step (lengths, starts, the block table) are read there.
+# that vary from step to step (lengths, starts, the block table) are read there.  Nothing is recorded for autograd.
 # ---------------------------------------------------------------------------------------------------------------------
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # TTSAMD_F32 / F16 / BF16
 
@@ -863,7 +863,8 @@ def _entry(what, arguments):
     """The library's function `what`: a packed struct, then `arguments` pointers and sizes."""
     fn = _FNS.get(what)
     if fn is None:
-        fn = getattr(lib(), "ttsamd_" + what)
+        fn = lib()["ttsamd_" + what]                # an object of its own: the library's attribute keeps taking the mirrors
+        fn.restype = getattr(lib(), "ttsamd_" + what).restype
         fn.argtypes = [ctypes.c_char_p] + [ctypes.c_void_p] * arguments
         _FNS[what] = fn
     return fn
@@ -944,6 +945,7 @@ class Rotary:
             if kind == "linear":
                 freq = [f / factor for f in freq]
             elif kind == "ramp":
+                _need("trained_len" in sc, "ramp: trained_len is wanted")
                 trained, low, high = float(sc.pop("trained_len")), float(sc.pop("low", 1.0)), float(sc.pop("high", 32.0))
                 _need(high > low, "ramp: high has to be above low")
                 keep = [min(1.0, max(0.0, (trained * f / (2 * math.pi) - low) / (high - low))) for f in freq]
@@ -1132,7 +1134,7 @@ class PackedW4:
     """A layer's 4-bit weights in the image the kernel streams (include/tts_amd.h, `ttsamd_linear_w4_args`).
 
     qweight uint8 [n, k / 2]: two levels 0..15 a byte, the even k in the low half; scales [n, k / group] in float32, float16 or bfloat16;
-    zeros uint8 [n, k / group] or None (8 everywhere); bias [n] or None.  group = k / scales.shape[1]: 32, 64 or 128.
+    zeros uint8 [n, k / group], 0..15, or None (8 everywhere); bias [n] or None.  group = k / scales.shape[1]: 32, 64 or 128.
     weight[n, k] = (level - zero) * scale.  Packing runs once, on the tensors' device."""
 
     def __init__(self, qweight, scales, zeros=None, bias=None):
