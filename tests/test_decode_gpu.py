@@ -235,6 +235,37 @@ def test_paged_attention(gpu, dtype, new, lens, kv, heads, dim, page):
     c.check(got, scale=0.3, window=max(1, max(lens) // 3), what="window")
 
 
+# heads between the widths that are powers of two, whole and in part
+BETWEEN = [
+    ([1, 1], [700, 33], 2, 4, 16), ([1], [3000], 1, 8, 32), ([9, 0, 2], [100, 40, 2], 1, 3, 1), ([129, 64, 1], [129, 190, 400], 2, 4, 16),
+    ([70, 90], [70, 350], 16, 64, 24), ([300], [1200], 1, 1, 13), ([130, 70, 5], [130, 200, 40], 64, 64, 16)]
+
+
+@pytest.mark.parametrize("dim", [88, 96, 136, 192])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("new,lens,kv,heads,page", BETWEEN)
+def test_paged_attention_heads_between_the_widths(gpu, dtype, dim, new, lens, kv, heads, page):
+    c = Case(gpu, dtype, new, lens, kv, heads, dim, page, seed=sum(lens) + dim, trailing=2)
+    c.check(ops.paged_attention(c.q.to(gpu), c.cache, c.batch), what="causal")
+    c.check(ops.paged_attention(c.q.to(gpu), c.cache, c.batch, window=60, scale=-0.1), scale=-0.1, window=60, what="window")
+
+
+@pytest.mark.parametrize("dim,heads", [(96, 2), (192, 2), (192, 1)])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_paged_attention_non_finite_values_between_the_widths(gpu, dtype, dim, heads):
+    """An infinity and a NaN that only the last tokens of a chunk see."""
+    new, n = 80, 200
+    c = Case(gpu, dtype, [new], [n], 1, heads, dim, 8, seed=3)
+    for j, value in ((n - 10, math.inf), (n - 6, math.nan)):
+        c.cache.v[int(c.table[0, j // 8]), :, j % 8, dim - 1] = value
+    got = ops.paged_attention(c.q.to(gpu), c.cache, c.batch).cpu()
+    want, _, _ = c.want(dim ** -0.5, True, 0)
+    assert torch.equal(torch.isfinite(got), torch.isfinite(want)) and bool(torch.isfinite(want[: new - 10]).all())
+    assert not bool(torch.isfinite(got[new - 10:, :, dim - 1]).any())
+    sub = got[: new - 10].double() - want[: new - 10]
+    assert float(sub.abs().max()) < 40 * u(dtype) + 1e-5
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("new,lens,window,kv", [([1, 1], [200, 33], 0, 2), ([40, 3], [200, 33], 0, 2), ([40, 90], [200, 90], 50, 2), ([1], [90], 1, 2),
                                                 ([140, 65], [200, 90], 50, 2), ([170], [840], 0, 2)])

@@ -15,20 +15,23 @@ PagedLaunch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv 
     PagedLaunch p = {};
     const bool f32 = c.dtype == TTSAMD_F32;
     const int group = a.q_heads / c.kv_heads;
-    p.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
+    // Heads between the widths of a power of two have kernels of their own (computed as 256 and 128: 48 single bf16 tokens over 2000 keys of
+    // 8 heads of 192 158 -> 112 us; chunks of 2 x 1024 tokens over 2048 keys, 32 heads over 8: bf16 of 192 299 -> 171, of 96 87 -> 82,
+    // fp32 of 192 1489 -> 469, of 96 333 -> 283; streamed, 96 are computed as 128: they wait for memory either way).
+    p.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : c.head_dim <= 192 ? 192 : 256;
     const int64_t rows = (int64_t)(b.max_new < 1 ? 1 : b.max_new) * group;
     const int64_t room = (int64_t)b.table_width * c.page_size;
     int64_t keys = b.max_len > 0 && b.max_len < room ? b.max_len : room;
     if (a.window > 0 && (int64_t)a.window + b.max_new < keys) keys = (int64_t)a.window + b.max_new;
     // Staged from some rows on (one sequence over 4096 keys; 8 key heads of 128, bf16: 128 / 256 / 1024 rows streamed 28.5 / 30.6 / 57 us,
     // staged 24.6 / 27.2 / 40; 16 of 64, fp32, 2048 keys: 64 / 128 / 256 rows streamed 20.1 / 25.0 / 35, staged 21.5 / 22.9 / 28.6).
-    p.tile = f32 ? p.dp <= 128 && rows >= (p.dp == 64 ? 96 : 64) : rows >= 96;
+    p.tile = f32 ? p.dp <= 192 && rows >= (p.dp == 64 ? 96 : 64) : rows >= 96;
     // One or two fp32 rows go without the matrix unit (one token over 605 keys of 16 heads of 64: 11.4 -> 8.0 us, 48 of up to 1007 keys: 59 ->
     // 56 us; heads over 128 channels would need more registers than they have).
     p.few = f32 && rows <= 2 && p.dp <= 128;
-    p.nq = p.few ? (int)rows : rows > 16 && p.dp < 256 ? 2 : 1;
+    p.nq = p.few ? (int)rows : rows > 16 && p.dp <= 128 ? 2 : 1;
     const bool pairs = p.tile && (p.dp == 64 || (p.dp == 128 && !f32));               // registers and LDS for two teams
-    const int kt = p.tile ? f32 ? kTile3Keys : kTileKeys : f32 || p.dp > 128 ? 16 : 32;
+    const int kt = p.tile ? f32 ? kTile3Keys : kTileKeys : f32 || p.dp > 192 ? 16 : 32;
     const int64_t key_tiles = keys < 1 ? 1 : (keys + kt - 1) / kt;
     p.waves = 4;
     if (pairs) {
@@ -53,7 +56,7 @@ PagedLaunch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv 
     // tiles left to a wave 14.1 / 16.0 / 21.0 us; one fp32 token over 605, 4.8 tiles a wave: whole 8.0 us, two splits 9.1, over 2048: 17.6
     // and, eight splits, 12.2.)
     p.splits = 1;
-    const int waves_held = p.tile ? p.dp > 128 || (f32 && p.dp > 64) || (p.waves == 2 && (f32 || p.dp > 64)) ? 4 : 8 : p.few ? 16 : p.dp == 64 ? 12 : p.dp == 128 ? 8 : 4;
+    const int waves_held = p.tile ? p.dp > 128 || (f32 && p.dp > 64) || (p.waves == 2 && (f32 || p.dp > 64)) ? 4 : 8 : p.few ? 16 : p.dp == 64 ? 12 : p.dp <= 192 ? 8 : 4;
     const int resident = waves_held / (p.waves * p.teams);                                  // workgroups a compute unit holds, by registers and LDS
     const int64_t fill = (int64_t)kCus * (resident < 1 ? 1 : resident) / blocks, a_wave = p.tile ? p.teams : p.waves;
     const int64_t most = key_tiles / (a_wave * (p.tile || rows > 64 ? 4 : p.few || rows > 32 ? 2 : 1));       // the join costs by the row
@@ -64,6 +67,7 @@ PagedLaunch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv 
     if ((int64_t)p.splits * c.kv_heads > 65535) p.splits = 65535 / c.kv_heads > 1 ? 65535 / c.kv_heads : 1;
     const int64_t each = (key_tiles + p.splits - 1) / p.splits;
     p.split_keys = (int)(each * kt < 0x7fffffff ? each * kt : 0x7fffffff);
+    if (p.tile && p.dp == 128 && c.head_dim <= 96) p.dp = 96;
     if (p.splits > 1) {
         const size_t n = (size_t)a.tokens * a.q_heads * p.splits;
         p.part_bytes = n * c.head_dim * sizeof(float), p.stat_bytes = n * 2 * sizeof(float);

@@ -18,32 +18,32 @@ template <class T, int DP, int NQ> hipError_t start_stream(const AttArgs &g, con
     return g.c.head_dim == DP ? start_stream<T, DP, NQ, true>(g, p, grid, st) : start_stream<T, DP, NQ, false>(g, p, grid, st);
 }
 
-template <class T, int DP, bool FULL, int RW, int KG> hipError_t start_tile(const AttArgs &g, dim3 grid, hipStream_t st)
+template <class T, int DC, bool FULL, int RW, int KG> hipError_t start_tile(const AttArgs &g, dim3 grid, hipStream_t st)
 {
     static std::atomic<unsigned long long> done{0};
-    constexpr int join = KG == 2 ? RW * (DP / 2 + 2) * 64 * 4 : 0;
+    constexpr int join = KG == 2 ? RW * (DC / 2 + 2) * 64 * 4 : 0;
     if constexpr (sizeof(T) == 4) {
-        constexpr int tiles = KG * 2 * 6 * kTile3Keys * DP * 2, bytes = tiles > join ? tiles : join;
-        if (hipError_t e = ensure_dynamic_lds((const void *)attend_tile3<DP, FULL, RW, KG>, bytes, done)) return e;
-        attend_tile3<DP, FULL, RW, KG><<<grid, 64 * RW * KG, bytes, st>>>(g);
+        constexpr int tiles = KG * 2 * 6 * kTile3Keys * tile3_pitch(DC) * 2, bytes = tiles > join ? tiles : join;
+        if (hipError_t e = ensure_dynamic_lds((const void *)attend_tile3<DC, FULL, RW, KG>, bytes, done)) return e;
+        attend_tile3<DC, FULL, RW, KG><<<grid, 64 * RW * KG, bytes, st>>>(g);
     } else {
-        constexpr int tiles = KG * 2 * 2 * kTileKeys * DP * 2, bytes = tiles > join ? tiles : join;
-        if (hipError_t e = ensure_dynamic_lds((const void *)attend_tile<T, DP, FULL, RW, KG>, bytes, done)) return e;
-        attend_tile<T, DP, FULL, RW, KG><<<grid, 64 * RW * KG, bytes, st>>>(g);
+        constexpr int tiles = KG * 2 * 2 * kTileKeys * padded_pow2(DC) * 2, bytes = tiles > join ? tiles : join;
+        if (hipError_t e = ensure_dynamic_lds((const void *)attend_tile<T, DC, FULL, RW, KG>, bytes, done)) return e;
+        attend_tile<T, DC, FULL, RW, KG><<<grid, 64 * RW * KG, bytes, st>>>(g);
     }
     return hipSuccess;
 }
-template <class T, int DP, int RW, int KG> hipError_t start_tile(const AttArgs &g, dim3 grid, hipStream_t st)
+template <class T, int DC, int RW, int KG> hipError_t start_tile(const AttArgs &g, dim3 grid, hipStream_t st)
 {
-    return g.c.head_dim == DP ? start_tile<T, DP, true, RW, KG>(g, grid, st) : start_tile<T, DP, false, RW, KG>(g, grid, st);
+    return g.c.head_dim == DC ? start_tile<T, DC, true, RW, KG>(g, grid, st) : start_tile<T, DC, false, RW, KG>(g, grid, st);
 }
-template <class T, int DP> hipError_t start_tile(const AttArgs &g, const PagedLaunch &p, dim3 grid, hipStream_t st)
+template <class T, int DC> hipError_t start_tile(const AttArgs &g, const PagedLaunch &p, dim3 grid, hipStream_t st)
 {
-    if constexpr (DP == 64 || (DP == 128 && sizeof(T) == 2)) {
-        if (p.waves == 2) return start_tile<T, DP, 2, 2>(g, grid, st);
-        if (p.teams == 2) return start_tile<T, DP, 4, 2>(g, grid, st);
+    if constexpr (DC == 64 || (DC <= 128 && sizeof(T) == 2)) {
+        if (p.waves == 2) return start_tile<T, DC, 2, 2>(g, grid, st);
+        if (p.teams == 2) return start_tile<T, DC, 4, 2>(g, grid, st);
     }
-    return start_tile<T, DP, 4, 1>(g, grid, st);
+    return start_tile<T, DC, 4, 1>(g, grid, st);
 }
 
 template <int DP, bool FULL, int R> hipError_t start_few(const AttArgs &g, const PagedLaunch &p, dim3 grid, hipStream_t st)
@@ -65,13 +65,16 @@ template <class T> hipError_t start_paged(const AttArgs &g, const PagedLaunch &p
     const dim3 grid(g.c.kv_heads * p.splits, p.row_tiles, g.b.batch);
     if (p.tile) {
         if (p.dp == 64) return start_tile<T, 64>(g, p, grid, st);
+        if (p.dp == 96) return start_tile<T, 96>(g, p, grid, st);
         if (p.dp == 128) return start_tile<T, 128>(g, p, grid, st);
+        if (p.dp == 192) return start_tile<T, 192>(g, p, grid, st);
         if constexpr (sizeof(T) == 2) return start_tile<T, 256>(g, p, grid, st);
     }
     if constexpr (sizeof(T) == 4)
         if (p.few) return p.dp == 64 ? start_few<64>(g, p, grid, st) : start_few<128>(g, p, grid, st);
     if (p.dp == 64) return p.nq == 2 ? start_stream<T, 64, 2>(g, p, grid, st) : start_stream<T, 64, 1>(g, p, grid, st);
     if (p.dp == 128) return p.nq == 2 ? start_stream<T, 128, 2>(g, p, grid, st) : start_stream<T, 128, 1>(g, p, grid, st);
+    if (p.dp == 192) return start_stream<T, 192, 1>(g, p, grid, st);
     return start_stream<T, 256, 1>(g, p, grid, st);
 }
 

@@ -172,9 +172,9 @@ template <class T, int DP, int NQ, bool FULL, int MAXW>
 __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
 {
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr int ES = sizeof(T), RB = DP * ES, NS = RB / 64, NV = DP / 16, KT = F32 || DP > 128 ? 16 : 32, NT = KT / 16;
+    constexpr int ES = sizeof(T), RB = DP * ES, NS = RB / 64, NV = DP / 16, KT = F32 || DP > 192 ? 16 : 32, NT = KT / 16;
     constexpr int VK = KT / 4;                          // values (keys) a lane holds of a tile
-    constexpr int VB = NV * ES, VP = VB < 16 ? 8 : 16;  // bytes of a lane's channels of one key, and of one load
+    constexpr int VB = NV * ES, VP = VB % 16 ? 8 : 16;  // bytes of a lane's channels of one key, and of one load
     extern __shared__ float lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int c16 = lane & 15, g4 = lane >> 4;
@@ -262,7 +262,7 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
                     const int at = c16 * VB + x * VP, in = FULL || at < D * ES ? at : 0;
                     if constexpr (VP == 8) {
                         const uint2 w = *(const uint2 *)(p + in);
-                        v[e][0] = w.x, v[e][1] = w.y;
+                        v[e][2 * x] = w.x, v[e][2 * x + 1] = w.y;
                     } else {
                         const uint4 w = *(const uint4 *)(p + in);
                         v[e][4 * x] = w.x, v[e][4 * x + 1] = w.y, v[e][4 * x + 2] = w.z, v[e][4 * x + 3] = w.w;

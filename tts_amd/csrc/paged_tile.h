@@ -45,10 +45,11 @@ template <int ND> __device__ __forceinline__ void join_teams(float *lds, int tea
     }
 }
 
-template <class T, int DP, bool FULL, int RW, int KG>
-__global__ __launch_bounds__(64 * RW * KG, DP > 128 || (DP == 128 && RW == 2) ? 1 : 2) void attend_tile(AttArgs g)
+template <class T, int DC, bool FULL, int RW, int KG>
+__global__ __launch_bounds__(64 * RW * KG, DC > 128 || (DC > 64 && RW == 2) ? 1 : 2) void attend_tile(AttArgs g)
 {
-    constexpr int CH = DP / 8, RB = DP * 2, NSTG = CH / RW, kTileRows = 32 * RW, RPI = 64 / CH, NS = DP / 16, ND = DP / 32, AHEAD = 4;
+    // DC channels are computed, of rows of DP in LDS
+    constexpr int DP = padded_pow2(DC), CH = DP / 8, RB = DP * 2, NSTG = CH / RW, kTileRows = 32 * RW, RPI = 64 / CH, NS = DC / 16, ND = DC / 32, AHEAD = 4;
     constexpr int HALF = kTileKeys * RB;                    // bytes of a tile's keys (or values)
     extern __shared__ float lds_f[];
     char *const lds = (char *)lds_f;
@@ -66,7 +67,8 @@ __global__ __launch_bounds__(64 * RW * KG, DP > 128 || (DP == 128 && RW == 2) ? 
 
     // staging: this thread's piece of NSTG rows
     const int piece = lane % CH, row_of_lane = lane / CH;
-    const bool piece_in = FULL || piece * 8 < D;
+    constexpr bool WHOLE = FULL && DC == DP;
+    const bool piece_in = WHOLE || piece * 8 < D;
     const char *kbase_l = kbase + (piece_in ? piece * 16 : 0), *vbase_l = vbase + (piece_in ? piece * 16 : 0);
     // reading: a key row per lane; four value rows and a 32-byte span per 16 lanes
     const int i16 = lane & 15, vr = 4 * h2 + (i16 >> 2), vc = 2 * (lane >> 4 & 1) + (i16 >> 1 & 1), vb8 = (i16 & 1) * 8;
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(64 * RW * KG, DP > 128 || (DP == 128 && RW == 2) ? 
 #pragma unroll
             for (int x = 0; x < NSTG; ++x) {
                 const int r = (x * RW + wave) * RPI + row_of_lane;
-                if (!FULL && !piece_in) st[x] = uint4{0, 0, 0, 0};
+                if (!WHOLE && !piece_in) st[x] = uint4{0, 0, 0, 0};
                 *(uint4 *)(buf + r * RB + ((piece ^ k_swz(r)) & (CH - 1)) * 16) = st[x];
             }
         };
@@ -128,7 +130,7 @@ __global__ __launch_bounds__(64 * RW * KG, DP > 128 || (DP == 128 && RW == 2) ? 
 #pragma unroll
             for (int x = 0; x < NSTG; ++x) {
                 const int r = (x * RW + wave) * RPI + row_of_lane;
-                if (!FULL && !piece_in) st[x] = uint4{0, 0, 0, 0};
+                if (!WHOLE && !piece_in) st[x] = uint4{0, 0, 0, 0};
                 *(uint4 *)(buf + HALF + r * RB + ((piece ^ v_swz(r)) & (CH - 1)) * 16) = st[x];
             }
         };

@@ -50,9 +50,12 @@ __device__ __forceinline__ f32x16_t mfma_three(const uint4 (&a)[3], const uint4 
     return mfma_32x32x16<__bf16>(a[0], b[0], c);
 }
 
-template <int DP, bool FULL, int RW, int KG> __global__ __launch_bounds__(64 * RW * KG, DP > 64 ? 1 : 2) void attend_tile3(AttArgs g)
+template <int DC, bool FULL, int RW, int KG> __global__ __launch_bounds__(64 * RW * KG, DC > 64 ? 1 : 2) void attend_tile3(AttArgs g)
 {
-    constexpr int CH = DP / 8, RB = DP * 2, PLANE = kTile3Keys * RB, NST = kTile3Keys * CH / (64 * RW), kTileRows = 32 * RW, NS = DP / 16, ND = DP / 32;
+    // DC channels are computed, of rows of DP in LDS
+    constexpr int DP = tile3_pitch(DC), CH = DP / 8, RB = DP * 2, PLANE = kTile3Keys * RB, NST = kTile3Keys * CH / (64 * RW), kTileRows = 32 * RW, NS = DC / 16,
+                  ND = DC / 32;
+    constexpr bool WHOLE = FULL && DC == DP;
     extern __shared__ float lds_f[];
     char *const lds = (char *)lds_f;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % RW), c32 = lane & 31, h2 = lane >> 5;
@@ -63,8 +66,9 @@ template <int DP, bool FULL, int RW, int KG> __global__ __launch_bounds__(64 * R
     const int D = g.c.head_dim, rows = s.n * g.group, tiles = (rows + kTileRows - 1) / kTileRows;
     const char *kbase = (const char *)g.c.k + (int64_t)hk * g.c.k_head * 4, *vbase = (const char *)g.c.v + (int64_t)hk * g.c.v_head * 4;
     const uint32_t page16 = (uint32_t)((h2 ? g.c.v_page : g.c.k_page) / 4), row16 = (uint32_t)((h2 ? g.c.v_row : g.c.k_row) / 4);
-    auto k_swz = [](int row) { return CH == 8 ? (row & 7) ^ (row >> 3 & 1) : row & 15; };
-    auto v_swz = [](int row) { return CH == 8 ? (row & 3) << 1 : (row & 1) << 2 | (row & 2) * 5; };
+    // within eight pieces where their number is no power of two (rows of 192 channels start at two places of the banks in turn)
+    auto k_swz = [](int row) { return CH == 8 ? (row & 7) ^ (row >> 3 & 1) : CH == 16 ? row & 15 : row >> 1 & 7; };
+    auto v_swz = [](int row) { return CH == 8 ? (row & 3) << 1 : CH == 16 ? (row & 1) << 2 | (row & 2) * 5 : (row & 2) << 1; };
     const int i16 = lane & 15, vr = 4 * h2 + (i16 >> 2), vc = 2 * (lane >> 4 & 1) + (i16 >> 1 & 1), vb8 = (i16 & 1) * 8;
     const float flip = g.scale2 < 0.f ? -1.f : g.scale2 == 0.f ? 0.f : 1.f, scale2 = g.scale2 == 0.f ? 1.f : fabsf(g.scale2);
 
@@ -105,7 +109,7 @@ template <int DP, bool FULL, int RW, int KG> __global__ __launch_bounds__(64 * R
             const uint32_t off = page < 0 ? 0 : (uint32_t)page * page16 + (uint32_t)row * row16;      // keys in lanes 0-31, values in 32-63
 #pragma unroll
             for (int x = 0; x < NST; ++x) {
-                const int i = x * 64 * RW + member, r = i / CH, piece = i % CH, at = FULL || piece * 8 < D ? piece * 32 : 0;
+                const int i = x * 64 * RW + member, r = i / CH, piece = i % CH, at = WHOLE || piece * 8 < D ? piece * 32 : 0;
                 const uint4 *ks = (const uint4 *)(kbase + (uint64_t)(uint32_t)__shfl((int)off, r) * 16 + at);
                 const uint4 *vs = (const uint4 *)(vbase + (uint64_t)(uint32_t)__shfl((int)off, 32 + r) * 16 + at);
                 sk[x][0] = ks[0], sk[x][1] = ks[1], sv[x][0] = vs[0], sv[x][1] = vs[1];
@@ -115,14 +119,14 @@ template <int DP, bool FULL, int RW, int KG> __global__ __launch_bounds__(64 * R
 #pragma unroll
             for (int x = 0; x < NST; ++x) {
                 const int i = x * 64 * RW + member, r = i / CH, piece = i % CH;
-                if (!(ok >> r & 1) || (!FULL && piece * 8 >= D)) sk[x][0] = sk[x][1] = sv[x][0] = sv[x][1] = uint4{0, 0, 0, 0};
+                if (!(ok >> r & 1) || (!WHOLE && piece * 8 >= D)) sk[x][0] = sk[x][1] = sv[x][0] = sv[x][1] = uint4{0, 0, 0, 0};
                 uint4 part[3];
                 split3(sk[x][0], sk[x][1], part, left);
 #pragma unroll
-                for (int p = 0; p < 3; ++p) *(uint4 *)(buf + p * PLANE + r * RB + ((piece ^ k_swz(r)) & (CH - 1)) * 16) = part[p];
+                for (int p = 0; p < 3; ++p) *(uint4 *)(buf + p * PLANE + r * RB + (piece ^ k_swz(r)) * 16) = part[p];
                 split3(sv[x][0], sv[x][1], part, left);
 #pragma unroll
-                for (int p = 0; p < 3; ++p) *(uint4 *)(buf + (3 + p) * PLANE + r * RB + ((piece ^ v_swz(r)) & (CH - 1)) * 16) = part[p];
+                for (int p = 0; p < 3; ++p) *(uint4 *)(buf + (3 + p) * PLANE + r * RB + (piece ^ v_swz(r)) * 16) = part[p];
             }
         };
 
