@@ -5,15 +5,19 @@
 // pairs come out).  The matrix unit sums x (16 + q) over a group in fp32, and x -(16 + z) beside it (a right operand of one value), and
 // the group's scale multiplies what that leaves: no product is rounded before the sum, and what cancels is at most some six times the
 // result's own size.
-// fp32 rows travel as three bf16 parts cut off one after the other (8 + 8 + 8 bits: exact), three products each.
+// fp32 rows travel as three bf16 parts cut off one after the other (8 + 8 + 8 bits: exact), three products each; up to five rows put their
+// parts beside each other into the sixteen rows of one product (8128 -> 1688, one row: 12.3 -> 10.0 us).
 //
 // Layout.  16x16x32 products with x as the left operand and 16 outputs as the right one: a lane holds the word of 8 levels of output
 // lane % 16, and 16 bytes of the image are the lane's words of four products (128 k): whole lines, read once, straight into registers.
-// x needs no staging either: the lane's eight k are neighbours in memory.  Row r of the left operand is row 4 (r % 4) + r / 4 of x, so
-// that up to four rows land in one accumulator register of every lane.
+// x goes through LDS, each wave its own chunk: the lanes of a product hold 16 rows each, and loads of 16 bytes a row cost a line each
+// (8128 -> 1688 with 16 rows, fp16 10.6 -> 7.6 us, fp32 17.6 -> 13.9).  Row r of the left operand is row 4 (r % 4) + r / 4 of x, so that
+// up to four rows land in one accumulator register of every lane.
 // A workgroup owns 16 outputs; its waves take the chunks of 128 k in turn and are joined in LDS.
 //
-// Bound: HBM by its bytes (0.5 + scale / group a weight) once the layer is large, the latency of one workgroup for small layers.
+// Bound: HBM by its bytes (0.5 + scale / group a weight) once the layer is large (8192 x 8192, group 128, one fp16 row: 34.6 MB in 8.4 us,
+// 4.1 TB/s), the latency of one workgroup for small layers (1024 x 1024: 3.0 us), unpacking and products from some 16 rows on (64 rows of
+// 8192 x 8192: 30 us, 280 TFLOP/s).
 #include "decode_common.h"
 
 namespace ttsamd {
@@ -63,15 +67,19 @@ template <class T, int GROUP> __device__ float summed(const ttsamd_linear_w4_arg
     return y;
 }
 
-template <class T, int NT, int GROUP, int MAXW> __global__ __launch_bounds__(MAXW * 64) void linear_w4(ttsamd_linear_w4_args a)
+// Rows of x that a wave stages a chunk of at most; of few rows, so many that a load each (16 bits) or three of them hold them.
+template <class T> constexpr int staged_rows(bool few) { return !few ? 16 : sizeof(T) == 4 ? 6 : 4; }
+template <class T> constexpr int few_rows() { return sizeof(T) == 4 ? 5 : 4; }
+
+template <class T, int NT, int GROUP, int MAXW, bool FEW> __global__ __launch_bounds__(MAXW * 64) void linear_w4(ttsamd_linear_w4_args a)
 {
-    constexpr bool F32 = sizeof(T) == 4, BF = !__is_same(T, _Float16);
-    constexpr int PARTS = F32 ? 3 : 1, PER = GROUP / 32, GPC = 128 / GROUP;      // products a group, groups a chunk
-    constexpr int RAW = F32 ? 2 : 1;                                             // 16-byte pieces of eight k of x
-    constexpr bool XAHEAD = !F32 && NT < 4;
+    constexpr bool F32 = sizeof(T) == 4, BF = !__is_same(T, _Float16), BESIDE = F32 && FEW;
+    constexpr int PARTS = F32 && !BESIDE ? 3 : 1, PER = GROUP / 32, GPC = 128 / GROUP;      // products a group, groups a chunk
+    constexpr int ES = sizeof(T), PPR = 8 * ES, RPI = 64 / PPR, XI = staged_rows<T>(FEW) / RPI;   // 16-byte pieces of a chunk of a row; rows a load; loads
+    constexpr bool XAHEAD = NT < 4 && !(F32 && !FEW && NT == 2 && GROUP == 32);          // the others have no registers left for it
     extern __shared__ float join[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int chunks = (a.k + 127) / 128, m0 = blockIdx.y * 16, rows = min(a.m - m0, 16);
+    const int chunks = (a.k + 127) / 128, m0 = blockIdx.y * 16, rows = min(a.m - m0, 16), products = BESIDE ? 3 * rows : rows;
     const int c16 = lane & 15, g4 = lane >> 4, row = 4 * (c16 & 3) + (c16 >> 2);
     unsigned one = BF ? 0x41804180u : 0x4c004c00u;
     asm("" : "+v"(one));
@@ -84,7 +92,10 @@ template <class T, int NT, int GROUP, int MAXW> __global__ __launch_bounds__(MAX
         sg[u] = tile * chunks * GPC * 16 + c16;
     }
     // a row behind the last is the last one again: no row of a product meets another
-    const T *const xrow = (const T *)a.x + (int64_t)(m0 + min(row, rows - 1)) * a.x_stride;
+    const T *const x0 = (const T *)a.x + (int64_t)m0 * a.x_stride;
+    const int piece = lane % PPR, lrow = lane / PPR, arow = min(BESIDE ? row / 3 : row, rows - 1);
+    char *const stage = (char *)join + wave * XI * RPI * 16 * PPR;
+    const unsigned first = BESIDE && row % 3 > 0 ? 0xffff0000u : 0u, second = BESIDE && row % 3 > 1 ? 0xffff0000u : 0u;     // parts that go before
     f32x4 acc[NT];
 #pragma unroll
     for (int u = 0; u < NT; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -93,12 +104,12 @@ template <class T, int NT, int GROUP, int MAXW> __global__ __launch_bounds__(MAX
     struct Chunk {
         uint4 word[NT];
         unsigned scale[NT][GPC], zero[NT][GPC];
-        uint4 x[XAHEAD ? 4 : 1][RAW];
+        uint4 x[XAHEAD ? XI : 1];
     } ahead[2];
     const bool wide = a.scale_dtype == TTSAMD_F32, brain = a.scale_dtype == TTSAMD_BF16, zeros = a.zeros != nullptr;
-    auto fetch_x = [&](uint4(&to)[RAW], int c, int j) {
-        const int k = 128 * c + 32 * j + 8 * g4;                                 // behind the last k the weights are 0: any x will do
-        __builtin_memcpy(to, xrow + (128 * c + 128 <= a.k ? k : min(k, a.k - 8)), 16 * RAW);
+    auto fetch_x = [&](uint4 &to, int c, int i) {
+        const int k = 128 * c + 16 / ES * piece;                                 // behind the last k the weights are 0: any x will do
+        __builtin_memcpy(&to, x0 + (int64_t)min(RPI * i + lrow, rows - 1) * a.x_stride + min(k, a.k - 16 / ES), 16);
     };
     auto fetch = [&](Chunk &f, int c) {
 #pragma unroll
@@ -113,12 +124,20 @@ template <class T, int NT, int GROUP, int MAXW> __global__ __launch_bounds__(MAX
         }
         if constexpr (XAHEAD)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) fetch_x(f.x[j], c, j);
+            for (int i = 0; i < XI; ++i) fetch_x(f.x[i], c, i);
     };
     auto multiply = [&](Chunk &f, int c) {
         unsigned word[NT][4], zero[NT][GPC];
         float scale[NT][GPC];
-        uint4 raw[4][RAW];
+        // x by way of LDS: loaded as it lies (whole lines), read as the products take it
+#pragma unroll
+        for (int i = 0; i < XI; ++i) {
+            const int r = RPI * i + lrow;
+            uint4 w;
+            if constexpr (XAHEAD) w = f.x[i];
+            else fetch_x(w, c, i);
+            *(uint4 *)(stage + r * 16 * PPR + (piece ^ r) * 16) = w;
+        }
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
             word[u][0] = f.word[u].x, word[u][1] = f.word[u].y, word[u][2] = f.word[u].z, word[u][3] = f.word[u].w;
@@ -132,19 +151,26 @@ template <class T, int NT, int GROUP, int MAXW> __global__ __launch_bounds__(MAX
                 else zero[u][q] = (unsigned)__builtin_bit_cast(unsigned short, (_Float16)z) * 0x10001u;
             }
         }
-        if constexpr (XAHEAD)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int y = 0; y < RAW; ++y) raw[j][y] = f.x[j][y];
         if (c + 2 * waves < chunks) fetch(f, c + 2 * waves);
-        if constexpr (!XAHEAD)
+        uint4 raw[4][ES / 2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) fetch_x(raw[j], c, j);
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int y = 0; y < ES / 2; ++y) raw[j][y] = *(const uint4 *)(stage + arow * 16 * PPR + (((4 * j + g4) * (ES / 2) + y) ^ arow) * 16);
         uint4 x[4][PARTS];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if constexpr (F32) {
+                if constexpr (BESIDE) {
+                    unsigned e8[8] = {raw[j][0].x, raw[j][0].y, raw[j][0].z, raw[j][0].w, raw[j][1].x, raw[j][1].y, raw[j][1].z, raw[j][1].w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        e8[e] = __float_as_uint(__uint_as_float(e8[e]) - __uint_as_float(e8[e] & first));
+                        e8[e] = __float_as_uint(__uint_as_float(e8[e]) - __uint_as_float(e8[e] & second));
+                    }
+                    x[j][0] = uint4{uppers(e8[0], e8[1]), uppers(e8[2], e8[3]), uppers(e8[4], e8[5]), uppers(e8[6], e8[7])};
+                    continue;
+                }
                 unsigned e8[8] = {raw[j][0].x, raw[j][0].y, raw[j][0].z, raw[j][0].w, raw[j][1].x, raw[j][1].y, raw[j][1].z, raw[j][1].w};
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p) {
@@ -183,37 +209,47 @@ template <class T, int NT, int GROUP, int MAXW> __global__ __launch_bounds__(MAX
         if (c + waves < chunks) multiply(ahead[1], c + waves);
     }
     // join the waves: [wave][x row][output]
+    __syncthreads();
     constexpr int LD = 16 * NT + 1;
 #pragma unroll
     for (int u = 0; u < NT; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (4 * i + g4 < rows) join[(wave * rows + 4 * i + g4) * LD + 16 * u + c16] = acc[u][i];
+            if (4 * i + g4 < products) join[(wave * products + 4 * i + g4) * LD + 16 * u + c16] = acc[u][i];
     __syncthreads();
     for (int it = threadIdx.x; it < rows * 16 * NT; it += blockDim.x) {
         const int r = it / (16 * NT), col = it % (16 * NT), n = blockIdx.x * 16 * NT + col;
         if (n >= a.n) continue;
         float y = a.bias ? to_f(((const T *)a.bias)[n]) : 0.f;
 #pragma unroll 4
-        for (int x = 0; x < waves; ++x) y += join[(x * rows + r) * LD + col];
+        for (int x = 0; x < waves; ++x) {
+            if constexpr (BESIDE) y += join[(x * products + 3 * r + 2) * LD + col] + join[(x * products + 3 * r + 1) * LD + col] + join[(x * products + 3 * r) * LD + col];
+            else y += join[(x * rows + r) * LD + col];
+        }
         if (!(fabsf(y) < __builtin_inff())) y = summed<T, GROUP>(a, m0 + r, n);
         ((T *)a.y)[(int64_t)(m0 + r) * a.y_stride + n] = (T)y;
     }
 }
 
-template <class T, int NT, int GROUP> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
+template <class T, int NT, int GROUP, bool FEW> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
 {
-    constexpr int MAXW = NT == 1 && sizeof(T) == 2 ? 16 : 8;
+    constexpr int MAXW = NT == 1 && sizeof(T) == 2 && FEW ? 16 : 8;
     const int chunks = (a.k + 127) / 128, blocks = (a.n + 16 * NT - 1) / (16 * NT), row_blocks = (a.m + 15) / 16;
     const bool few = (int64_t)blocks * row_blocks < 256;
-    // Waves share the chunks of k: eight, or sixteen where there are fewer workgroups than compute units.
+    // Waves share the chunks of k: eight, or sixteen where there are fewer workgroups than compute units (and the registers of few rows).
     int waves = MAXW > 8 && few ? 16 : 8;
     while (waves > 1 && waves > chunks) waves /= 2;
-    const int rows = a.m < 16 ? a.m : 16, bytes = waves * rows * (16 * NT + 1) * 4;
+    const int rows = a.m < 16 ? a.m : 16, joined = waves * (FEW && sizeof(T) == 4 ? 3 * rows : rows) * (16 * NT + 1) * 4;
+    constexpr int staged = staged_rows<T>(FEW) * 128 * (int)sizeof(T), most_joined = MAXW * 16 * (16 * NT + 1) * 4;
+    const int bytes = joined > waves * staged ? joined : waves * staged;
     static std::atomic<unsigned long long> done{0};
-    if (hipError_t e = ensure_dynamic_lds((const void *)linear_w4<T, NT, GROUP, MAXW>, MAXW * 16 * (16 * NT + 1) * 4, done)) return e;
-    linear_w4<T, NT, GROUP, MAXW><<<dim3(blocks, row_blocks), waves * 64, bytes, st>>>(a);
+    if (hipError_t e = ensure_dynamic_lds((const void *)linear_w4<T, NT, GROUP, MAXW, FEW>, most_joined > MAXW * staged ? most_joined : MAXW * staged, done)) return e;
+    linear_w4<T, NT, GROUP, MAXW, FEW><<<dim3(blocks, row_blocks), waves * 64, bytes, st>>>(a);
     return hipSuccess;
+}
+template <class T, int NT, int GROUP> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
+{
+    return a.m <= few_rows<T>() ? start<T, NT, GROUP, true>(a, st) : start<T, NT, GROUP, false>(a, st);
 }
 template <class T, int NT> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
 {
@@ -221,9 +257,10 @@ template <class T, int NT> hipError_t start(const ttsamd_linear_w4_args &a, hipS
 }
 template <class T> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
 {
-    // Every workgroup reads its rows of x whole: several output tiles a wave read them once, as long as the chip stays full and the
-    // registers hold (fp16, group 128: 8192 x 8192 with 16 rows 18.7 / 13.1 / 16.4 us at 1 / 2 / 4 tiles, with 64 rows 63 / 46 / 31 us;
-    // 4096 -> 2048, 32 rows: 6.8 / 7.6 / 9.0 us; bf16, group 32: 1024 -> 8192, 64 rows 15.2 / 12.9 / 16.1 us).
+    // Every workgroup reads its rows of x whole: several output tiles a wave read (and, fp32, split) them once, as long as the chip stays
+    // full and the registers hold (fp16, group 128: 8192 x 8192 with 16 rows 11.8 / 10.7 / 15.3 us at 1 / 2 / 4 tiles, with 64 rows 38.7 /
+    // 35.5 / 30.2 us; 4096 -> 2048, 32 rows: 5.1 / 6.1 / 8.5 us; bf16, group 32: 1024 -> 8192, 64 rows 15.9 / 13.2 / 16.2 us; fp32, 8192 x
+    // 8192 with one row 14.9 / 12.1 us).
     const int64_t tiles = (int64_t)((a.n + 15) / 16) * ((a.m + 15) / 16);
     if (tiles < 512) return start<T, 1>(a, st);
     if constexpr (sizeof(T) == 2)
