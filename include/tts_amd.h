@@ -707,8 +707,8 @@ typedef struct ttsamd_paged_kv {
 } ttsamd_paged_kv;
 /* The sequences of a call.  seq_lens[b] counts all tokens of sequence b, the new ones included: its new token i sits at position
  * p = seq_lens[b] - n_b + i, n_b = q_starts[b+1] - q_starts[b], in row p % page_size of page block_table[b][p / page_size].
- * max_new and max_len (0: what the table can hold) are what the launch is sized by (any n_b and length is still computed whole).  Everything is bounded on the
- * device: starts are clamped to the tokens of the call, and a position that is negative, behind the table's width or on a page
+ * max_new and max_len (0: what the table can hold) are what the launch is sized by (any n_b and length is still computed whole).
+ * Everything is bounded on the device: starts are clamped to the tokens of the call, and a position that is negative, behind the table's width or on a page
  * outside [0, pages) holds no key and takes no write (-1 marks a column without a page). */
 typedef struct ttsamd_paged_batch {
     const int32_t *block_table;           /* [batch, table_width], row stride table_stride */
@@ -755,8 +755,8 @@ int ttsamd_paged_attention(const ttsamd_paged_attention_args *args /* host */, c
 /* y[m, n] = sum_k x[m, k] * (level[n, k] - zero[n, k / group]) * scale[n, k / group] + bias[n]: a layer with 4-bit weights for the few
  * rows of a decoding step.  Levels and zeros 0..15; without zero points the zero is 8.  fp32 sums of exact products.
  * `levels`: the image [ceil(n/16)][ceil(k/128)][4 g][16 r][4 j] of 32-bit words; word (g, r, j) of tile (t, c) holds the levels of
- * output 16 t + r at k = 128 c + 32 j + 8 g + e, e = 0..7: level 2p from bit 4p, level 2p + 1 from bit 16 + 4p.  `scales` / `zeros`: [ceil(n/16)][groups of the
- * padded k][16 r], scales in scale_dtype, zeros uint8 (or NULL); padding has scale 0.  All three start at 16 bytes. */
+ * output 16 t + r at k = 128 c + 32 j + 8 g + e, e = 0..7: level 2p from bit 4p, level 2p + 1 from bit 16 + 4p.
+ * `scales` / `zeros`: [ceil(n/16)][groups of the padded k][16 r], scales in scale_dtype, zeros uint8 (or NULL); padding has scale 0.  All three start at 16 bytes. */
 typedef struct ttsamd_linear_w4_args {
     const void *x;                        /* [m, k], rows at x_stride */
     void *y;                              /* [m, n], rows at y_stride */

@@ -395,7 +395,10 @@ def _w4(dtype, m, n, k, group, zeros, bias, seed):
     (1, 1, 32, 32, False, False), (1, 16, 128, 128, True, True), (2, 100, 256, 64, False, True), (5, 17, 96, 32, True, False),
     (1, 1024, 1024, 64, False, True), (16, 33, 640, 128, True, True), (17, 64, 320, 64, False, False), (33, 250, 1056, 32, True, True),
     (64, 48, 512, 128, False, True), (100, 20, 192, 64, True, False), (1, 40, 8192, 128, False, True), (4, 4096, 64, 64, True, True),
-    (260, 70, 384, 128, False, False)])
+    (260, 70, 384, 128, False, False),
+    # few and many rows where a workgroup has two and four tiles of outputs, the last of them in part
+    (3, 8200, 96, 32, True, True), (5, 8199, 192, 64, False, True), (6, 8195, 160, 32, True, False), (16, 8200, 384, 128, True, True),
+    (1, 16400, 128, 64, True, False), (4, 16390, 640, 128, False, True), (2, 16386, 64, 32, False, False), (20, 8203, 320, 64, True, True)])
 def test_linear_w4(gpu, dtype, m, n, k, group, zeros, bias):
     x, q, s, z, b = _w4(dtype, m, n, k, group, zeros, bias, m + n + k)
     want, mag = O.linear_w4(x, q, s, z, b)

@@ -9,7 +9,8 @@
 // computed again key by key.
 //
 // Bound: the instructions issued, matrix ones (36 cycles each, 48 of them a wave for 32 keys of 64 channels) and others (4) one after
-// the other: about 3200 cycles, against 6200 with the fp32 products.
+// the other: about 3200 cycles, against 6200 with the fp32 products (one chunk of 700 tokens over 2048 keys, 16 heads of 64: 79 -> 53 us; two
+// ragged prompts of up to 437: 21 us).
 #pragma once
 #include "paged_tile.h"
 
