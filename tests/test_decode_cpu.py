@@ -191,7 +191,7 @@ def test_w4_image_holds_every_level_in_its_place():
 
 
 def test_oracle_against_plain_softmax():
-    """The 64-bit checker itself, on a batch whose pages lie in order: torch's own softmax."""
+    """The 64-bit oracle itself, on a batch whose pages lie in order: torch's own softmax."""
     g = torch.Generator().manual_seed(1)
     k, v = (torch.randn(4, 2, 8, 16, generator=g, dtype=torch.float64) for _ in range(2))
     q = torch.randn(3, 4, 16, generator=g, dtype=torch.float64)

@@ -26,7 +26,7 @@ PagedLaunch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv 
     // Staged from some rows on (one sequence over 4096 keys; 8 key heads of 128, bf16: 128 / 256 / 1024 rows streamed 28.5 / 30.6 / 57 us,
     // staged 24.6 / 27.2 / 40; 16 of 64, fp32, 2048 keys: 64 / 128 / 256 rows streamed 20.1 / 25.0 / 35, staged 21.5 / 22.9 / 28.6).
     p.tile = f32 ? p.dp <= 192 && rows >= (p.dp == 64 ? 96 : 64) : rows >= 96;
-    // One or two fp32 rows go without the matrix unit (one token over 605 keys of 16 heads of 64: 11.4 -> 8.0 us, 48 of up to 1007 keys: 59 ->
+    // One or two fp32 rows go without the matrix unit (one token over 605 keys of 16 heads of 64: 11.4 -> 7.6 us, 48 of up to 1007 keys: 59 ->
     // 56 us; heads over 128 channels would need more registers than they have).
     p.few = f32 && rows <= 2 && p.dp <= 128;
     p.nq = p.few ? (int)rows : rows > 16 && p.dp <= 128 ? 2 : 1;

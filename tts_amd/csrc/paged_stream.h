@@ -24,6 +24,8 @@
 // Bound: HBM for single tokens.  48 fp16 sequences of up to 1007 keys, 16 heads of 64: 150 MB in 31.5 us (4.8 TB/s); three bf16 ones of up
 // to 65537, 32 heads over 4 of 128: 363 MB in 66 us (5.5 TB/s; a large copy reaches 5.0 to 5.3), and 5 for the join of 21 splits.
 #pragma once
+#include <type_traits>
+
 #include "decode_common.h"
 
 namespace ttsamd {
@@ -407,7 +409,7 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
 }
 
 // One or two fp32 rows: the same stream without the matrix unit, whose fp32 products of 16 rows would leave 14 of them idle at 1152 cycles
-// a tile of 16 keys of 64 channels, against some 360 here (one token over 605 keys of 16 heads of 64: 8.0 us, latency).  A lane holds
+// a tile of 16 keys of 64 channels, against some 330 here (one token over 605 keys of 16 heads of 64: 6.9 us a launch of a graph).  A lane holds
 // four channels of every 64 of keys 4 (lane / 16) + i: whole rows of 16 lanes add up a score by rotation, so that the lanes of a key know
 // it, and each 16 lanes keep a maximum, sum and output of their own until the end.
 template <int DP, bool FULL, int R> __global__ __launch_bounds__(512) void attend_few(AttArgs g)
@@ -425,13 +427,14 @@ template <int DP, bool FULL, int R> __global__ __launch_bounds__(512) void atten
     const float flip = g.scale2 < 0.f ? -1.f : g.scale2 == 0.f ? 0.f : 1.f, scale2 = g.scale2 == 0.f ? 1.f : fabsf(g.scale2);
     for (int r0 = blockIdx.y * R; r0 < rows; r0 += gridDim.y * R) {
         const int last = min(r0 + R, rows) - 1;
-        Range mine[R], all = {0x7fffffff, 0};
+        Range mine[R], all = {0x7fffffff, 0}, both = {0, 0x7fffffff};            // what some row sees, what every row sees
         f32x4_t q[R][NX];
 #pragma unroll
         for (int u = 0; u < R; ++u) {
             const int r = min(r0 + u, last), i = g.by_group.div(r), h = hk * g.group + r - i * g.group;
             mine[u] = seen_by(s, s.len - s.n + i, g.a.causal, g.a.window);
             all.begin = min(all.begin, mine[u].begin), all.end = max(all.end, mine[u].end);
+            both.begin = max(both.begin, mine[u].begin), both.end = min(both.end, mine[u].end);
             const float *src = (const float *)g.a.q + (int64_t)(s.start + i) * g.a.q_tstride + (int64_t)h * g.a.q_hstride;
 #pragma unroll
             for (int x = 0; x < NX; ++x) {
@@ -498,35 +501,40 @@ template <int DP, bool FULL, int R> __global__ __launch_bounds__(512) void atten
                     sc[u][i] = x;
                 }
             if (base + step < hi) load(k, kbase, off, 0);
+            auto add = [&](auto whole) {                       // whole: every row sees every key of the tile
+                constexpr bool ALL = decltype(whole)::value;
 #pragma unroll
-            for (int u = 0; u < R; ++u) {
-                const uint32_t bits = (uint32_t)seen_bits(ok_now, base, mine[u]) >> (4 * g4);
-                float top = kNoMax;
+                for (int u = 0; u < R; ++u) {
+                    const uint32_t bits = ALL ? ~0u : (uint32_t)seen_bits(ok_now, base, mine[u]) >> (4 * g4);
+                    float top = kNoMax;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    sc[u][i] = masked(sc[u][i], bits, i);
-                    top = fmaxf(top, sc[u][i] * scale2);
+                    for (int i = 0; i < 4; ++i) {
+                        if (!ALL) sc[u][i] = masked(sc[u][i], bits, i);
+                        top = fmaxf(top, sc[u][i] * scale2);
+                    }
+                    if (__any(top > m[u] + kLazy)) {
+                        const float to = fmaxf(m[u], top), fade = __builtin_amdgcn_exp2f(m[u] - to);
+                        m[u] = to, l[u] *= fade;
+#pragma unroll
+                        for (int x = 0; x < NX; ++x) o[u][x] *= fade;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][i], scale2, -m[u]));
+                        l[u] += p;
+#pragma unroll
+                        for (int x = 0; x < NX; ++x)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                // a key that is not seen takes no part, whatever its value holds
+                                const float value = ALL || (bits >> i & 1) ? v[i][x][e] : 0.f;
+                                o[u][x][e] = fmaf(p, value, o[u][x][e]);
+                            }
+                    }
                 }
-                if (__any(top > m[u] + kLazy)) {
-                    const float to = fmaxf(m[u], top), fade = __builtin_amdgcn_exp2f(m[u] - to);
-                    m[u] = to, l[u] *= fade;
-#pragma unroll
-                    for (int x = 0; x < NX; ++x) o[u][x] *= fade;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][i], scale2, -m[u]));
-                    l[u] += p;
-#pragma unroll
-                    for (int x = 0; x < NX; ++x)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            // a key that is not seen takes no part, whatever its value holds
-                            const float value = bits >> i & 1 ? v[i][x][e] : 0.f;
-                            o[u][x][e] = fmaf(p, value, o[u][x][e]);
-                        }
-                }
-            }
+            };
+            if (ok_now == 0xffffu && base >= both.begin && base + KT <= both.end) add(std::true_type());
+            else add(std::false_type());
         }
         // join the 16 lanes' results of a wave, then the waves
         constexpr int LDO = DP + 4;
