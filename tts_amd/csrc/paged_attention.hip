@@ -59,7 +59,13 @@ PagedLaunch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv 
     const int waves_held = p.tile ? p.dp > 128 || (f32 && p.dp > 64) || (p.waves == 2 && (f32 || p.dp > 64)) ? 4 : 8 : p.few ? 16 : p.dp == 64 ? 12 : p.dp <= 192 ? 8 : 4;
     const int resident = waves_held / (p.waves * p.teams);                                  // workgroups a compute unit holds, by registers and LDS
     const int64_t fill = (int64_t)kCus * (resident < 1 ? 1 : resident) / blocks, a_wave = p.tile ? p.teams : p.waves;
-    const int64_t most = key_tiles / (a_wave * (p.tile || rows > 64 ? 4 : p.few || rows > 32 ? 2 : 1));       // the join costs by the row
+    // Tiles left to a wave, or a team, of a split: the join costs by the row and the split.  Staged, at least 1 / 2 / 4: 24 workgroups of fp16
+    // rows (2 x 84 tokens, 8 heads over 4 of 128) over 600 keys 16.2 / 19.3 / 19.8 us, over 1815 19.6 / 21.2 / 24.7; 12 over 4096 (21 and 16
+    // splits) 21.3 / 18.7 / 22.1; 1600 rows of one head of 64 over 1815 16.4 / 14.8 / 16.3; 128 workgroups of 64 over 600 keys 14.9 / 14.0 /
+    // 13.0, over 1815 19.6 / 19.6 / 21.2.
+    const int least = p.tile ? blocks <= 32 && rows <= 512 ? 1 : blocks >= 64 && key_tiles <= 8 * a_wave ? 4 : 2 : rows > 64 ? 4 : p.few || rows > 32 ? 2 : 1;
+    int64_t most = key_tiles / (a_wave * least);
+    if (p.tile && least == 1 && most > 16) most = key_tiles / (2 * a_wave) > 16 ? key_tiles / (2 * a_wave) : 16;
     if (fill > 1 && key_tiles > (p.few ? 8 : 4) * a_wave) p.splits = (int)(fill < most ? fill : most);
     // Parts are laid out by the token, whoever owns it: a call whose tokens are mostly padding gets fewer splits, not gigabytes.
     const size_t rows_bytes = (size_t)a.tokens * a.q_heads * (c.head_dim + 2) * sizeof(float), room_bytes = (size_t)256 << 20;
