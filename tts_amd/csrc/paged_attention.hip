@@ -52,9 +52,9 @@ PagedLaunch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv 
     p.teams = pairs && (p.waves == 2 || (blocks <= kCus && key_tiles >= 4)) ? 2 : 1;
     // Still few, and long: the keys are split over workgroups until one round of them fills the chip, and a second launch joins them.
     // (Three tokens over 65537 keys, 12 workgroups of 8 waves, one a compute unit: 21 / 32 / 42 / 85 splits 70.6 / 84.0 / 75.5 / 87.2 us;
-    // one bf16 token over 605 keys, 2.4 tiles a wave: whole 8.2 us, two splits 11.0; one over 4096, 16 tiles a wave: at least 1 / 2 / 4
-    // tiles left to a wave 14.1 / 16.0 / 21.0 us; one fp32 token over 605, 4.8 tiles a wave: whole 8.0 us, two splits 9.1, over 2048: 17.6
-    // and, eight splits, 12.2.)
+    // one bf16 token over 605 keys, 2.4 tiles a wave: whole 8.2 us, two splits 11.0; 32 heads over 8 of 128, 600 keys 11.0 and 11.6, 1000
+    // 15.0 and 12.0; one over 4096, 16 tiles a wave: at least 1 / 2 / 4 tiles left to a wave 14.1 / 16.0 / 21.0 us; one fp32 token over 605,
+    // 4.8 tiles a wave: whole 8.0 us, two splits 9.1, over 2048: 17.6 and, eight splits, 12.2.)
     p.splits = 1;
     const int waves_held = p.tile ? p.dp > 128 || (f32 && p.dp > 64) || (p.waves == 2 && (f32 || p.dp > 64)) ? 4 : 8 : p.few ? 16 : p.dp == 64 ? 12 : p.dp <= 192 ? 8 : 4;
     const int resident = waves_held / (p.waves * p.teams);                                  // workgroups a compute unit holds, by registers and LDS
@@ -66,7 +66,7 @@ PagedLaunch plan_of(const ttsamd_paged_attention_args &a, const ttsamd_paged_kv 
     const int least = p.tile ? blocks <= 32 && rows <= 512 ? 1 : blocks >= 64 && key_tiles <= 8 * a_wave ? 4 : 2 : rows > 64 ? 4 : p.few || rows > 32 ? 2 : 1;
     int64_t most = key_tiles / (a_wave * least);
     if (p.tile && least == 1 && most > 16) most = key_tiles / (2 * a_wave) > 16 ? key_tiles / (2 * a_wave) : 16;
-    if (fill > 1 && key_tiles > (p.few ? 8 : 4) * a_wave) p.splits = (int)(fill < most ? fill : most);
+    if (fill > 1 && key_tiles > (p.few ? 8 : p.tile || p.dp == 64 ? 4 : 3) * a_wave && most > 1) p.splits = (int)(fill < most ? fill : most);
     // Parts are laid out by the token, whoever owns it: a call whose tokens are mostly padding gets fewer splits, not gigabytes.
     const size_t rows_bytes = (size_t)a.tokens * a.q_heads * (c.head_dim + 2) * sizeof(float), room_bytes = (size_t)256 << 20;
     if (p.splits * rows_bytes > room_bytes) p.splits = rows_bytes * 2 > room_bytes ? 1 : (int)(room_bytes / rows_bytes);
