@@ -190,6 +190,16 @@ def test_w4_image_holds_every_level_in_its_place():
                 assert int(pw.zeros[i // 16, j // group, i % 16]) == (int(z[i, j // group]) if inside else 0)
 
 
+def test_w4_image_is_its_own():
+    """One group of one chunk: the image's scales and zeros have the order of the given ones, but no memory in common with them."""
+    scales, zeros = torch.rand(33, 1)[1:], torch.full((33, 1), 3, dtype=torch.uint8)[1:]
+    pw = ops.PackedW4(torch.zeros(32, 64, dtype=torch.uint8), scales, zeros)
+    before = pw.scales.clone()
+    scales.zero_(), zeros.zero_()
+    assert torch.equal(pw.scales, before) and bool((pw.zeros == 3).all())
+    assert pw.scales.data_ptr() % 16 == 0 and pw.zeros.data_ptr() % 16 == 0
+
+
 def test_oracle_against_plain_softmax():
     """The 64-bit oracle itself, on a batch whose pages lie in order: torch's own softmax."""
     g = torch.Generator().manual_seed(1)

@@ -1163,7 +1163,7 @@ class PackedW4:
         self.levels = words.permute(0, 2, 4, 1, 3).contiguous()                          # [t, c, g, r, j]
 
         def by_group(t):
-            return padded(t, chunks * per).view(tiles, 16, chunks * per).transpose(1, 2).contiguous()
+            return padded(t, chunks * per).view(tiles, 16, chunks * per).transpose(1, 2).clone(memory_format=torch.contiguous_format)
 
         self.scales = by_group(scales)
         self.zeros = None if zeros is None else by_group(zeros)
