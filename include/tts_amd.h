@@ -737,7 +737,7 @@ int ttsamd_kv_append(const ttsamd_kv_append_args *args /* host */, const ttsamd_
 /* Attention of the new tokens over the cache: out[t,h] = softmax_j(scale * q[t,h] . k_j) v_j over the keys j of t's sequence that
  * hold a key, with j <= p when causal != 0 and j > p - window when window > 0; p = t's position.  Query head h reads key head
  * h / (q_heads / kv_heads).  A row that sees no key is zero.  Rows of `out` behind the last sequence are left as they were.
- * Statistics and sums in fp32.  head_dim a multiple of 8 up to 256; q, out and the cache start and stride at 16 bytes.
+ * Statistics and sums in fp32; scores up to 2^127 in size.  head_dim a multiple of 8 up to 256; q, out and the cache start and stride at 16 bytes.
  * `workspace` (device, ttsamd_paged_attention_workspace_bytes, at most 256 MiB; 16-byte aligned; nothing is kept in it between calls, and
  * no two calls that may run at once share one): partial results where a long cache is split over the chip. */
 typedef struct ttsamd_paged_attention_args {

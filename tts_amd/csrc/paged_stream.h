@@ -12,7 +12,7 @@
 // and regroups the halves with one v_perm per pair, so nothing passes through LDS.  fp32 uses the 4-deep fp32 product: no regrouping,
 // 16 keys a tile.
 //
-// The running maximum moves only when a score exceeds it by more than 2^8 (p <= 256 then, exact in every type's range): the cross-lane
+// The running maximum moves only when a score exceeds it by more than 2^8 (p <= 256 then, within every type's range): the cross-lane
 // maximum and the scaling of O are skipped in almost every tile.
 //
 // Where a tile's rows lie (page lookup, one key a lane, keys in lanes 0-31 and values in lanes 32-63) is fetched a tile ahead; a
@@ -35,7 +35,8 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
-constexpr float kNoMax = -1e38f;     // a running maximum before the first key: finite, so that no difference of two is NaN
+constexpr float kNoMax = -3.402823466e38f;      // a running maximum before the first key: no score lies below it, no difference of two is NaN
+constexpr float kFar = 4194304.f;               // 2^22
 constexpr float kLazy = 8.f;         // how far (log2) a score may exceed the running maximum before it moves
 
 struct AttArgs {
@@ -48,6 +49,12 @@ struct AttArgs {
     float *part;                     // splits > 1: [tokens * q_heads][splits][head_dim], then [tokens * q_heads][splits][2]
     float *stat;
 };
+
+// p = exp2(s scale2 - m) as one fma takes m, the rounded product of a largest score, from s scale2 unrounded: every p of the row is off by
+// the same power of two, half a last place of m at most, in whichever part of the keys it lies, and that falls out of o / l as long as it
+// is small.  From |m| = 2^22 on (a quarter) it need not be: for such rows (is_far) the scores are scaled and rounded as the maximum was
+// before it is taken away, and its key has p = 1.  Scores are to stay within 2^127 in size, so that their product with log2 e is finite.
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > kFar && m > kNoMax; }
 
 template <class T> __device__ __forceinline__ f32x4_t mfma_16x16x32(uint4 a, uint4 b, f32x4_t c);
 template <> __device__ __forceinline__ f32x4_t mfma_16x16x32<__bf16>(uint4 a, uint4 b, f32x4_t c)
@@ -118,7 +125,7 @@ __device__ float attend_row(const AttArgs &g, int b, int hk, const T *q, Range s
         float x = 0.f;
         for (int d = lane; d < D; d += 64) x = fmaf(to_f(q[d]), to_f(k[d]), x);
         for (int y = 32; y; y >>= 1) x += __shfl_xor(x, y);
-        const float to = fmaxf(m, x * g.scale2), fade = __builtin_amdgcn_exp2f(m - to), p = __builtin_amdgcn_exp2f(fmaf(x, g.scale2, -to));
+        const float t = x * g.scale2, to = fmaxf(m, t), fade = __builtin_amdgcn_exp2f(m - to), p = __builtin_amdgcn_exp2f(is_far(to) ? t - to : fmaf(x, g.scale2, -to));
         m = to, l = l * fade + p;
         for (int y = 0; y < 4; ++y)
             if (lane + 64 * y < D) acc[y] = fmaf(p, to_f(v[lane + 64 * y]), acc[y] * fade);
@@ -224,7 +231,7 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
             for (int x = 0; x < NV; ++x) o[u][x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         }
 
-        bool odd = false;
+        bool odd = false, far[NQ] = {};
         int base = lo + wave * KT;
         const int step = waves * KT, idx = lane & (KT - 1);
         uint4 k[NT][NS];
@@ -329,10 +336,18 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
                     m[u] = to, l[u] *= fade;
 #pragma unroll
                     for (int x = 0; x < NV; ++x) o[u][x] *= fade;
+                    far[u] = __any(is_far(to));
+                }
+                float by = scale2, off = m[u];
+                if (far[u]) {
+                    const bool it = is_far(m[u]);
+#pragma unroll
+                    for (int e = 0; e < VK; ++e) sc[u][e >> 2][e & 3] = it ? sc[u][e >> 2][e & 3] * scale2 - m[u] : sc[u][e >> 2][e & 3];
+                    if (it) by = 1.f, off = 0.f;
                 }
 #pragma unroll
                 for (int e = 0; e < VK; ++e) {
-                    p[u][e] = __builtin_amdgcn_exp2f(fmaf(sc[u][e >> 2][e & 3], scale2, -m[u]));
+                    p[u][e] = __builtin_amdgcn_exp2f(fmaf(sc[u][e >> 2][e & 3], by, -off));
                     if constexpr (F32) l[u] += p[u][e];
                 }
             }
@@ -454,6 +469,7 @@ template <int DP, bool FULL, int R> __global__ __launch_bounds__(512) void atten
         }
         const int step = waves * KT;
         int base = lo + wave * KT;
+        bool far[R] = {};
         auto fetch = [&](int at, int &row) { return entry_of(g.b, g.by_page, b, min(at + c16, hi - 1), row); };
         auto place = [&](int at, int entry) { return at + c16 < hi && held(entry, g.c.pages) ? entry : -1; };
         // keys in lanes 0-15, values in 32-47: where the four of this lane's sixteen lie
@@ -517,10 +533,18 @@ template <int DP, bool FULL, int R> __global__ __launch_bounds__(512) void atten
                         m[u] = to, l[u] *= fade;
 #pragma unroll
                         for (int x = 0; x < NX; ++x) o[u][x] *= fade;
+                        far[u] = __any(is_far(to));
+                    }
+                    float by = scale2, off = m[u];
+                    if (far[u]) {
+                        const bool it = is_far(m[u]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sc[u][i] = it ? sc[u][i] * scale2 - m[u] : sc[u][i];
+                        if (it) by = 1.f, off = 0.f;
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][i], scale2, -m[u]));
+                        const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][i], by, -off));
                         l[u] += p;
 #pragma unroll
                         for (int x = 0; x < NX; ++x)

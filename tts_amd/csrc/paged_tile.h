@@ -101,7 +101,7 @@ __global__ __launch_bounds__(64 * RW * KG, DC > 128 || (DC > 64 && RW == 2) ? 1 
 #pragma unroll
             for (int y = 0; y < 16; ++y) o[x][y] = 0.f;
         float m = kNoMax, l = 0.f;
-        bool odd = false;
+        bool odd = false, far = false;
 
         const int64_t from = first.begin + (int64_t)split * g.split_keys, to = split + 1 < g.splits ? from + g.split_keys : final.end;
         const int lo = (int)min(from, (int64_t)final.end), hi = (int)min(to, (int64_t)final.end);
@@ -211,6 +211,14 @@ __global__ __launch_bounds__(64 * RW * KG, DC > 128 || (DC > 64 && RW == 2) ? 1 
                     m = to, l *= fade;
 #pragma unroll
                     for (int x = 0; x < ND; ++x) o[x] *= fade;
+                    far = __any(is_far(to));
+                }
+                float by = scale2, off = m;
+                if (far) {
+                    const bool it = is_far(m);
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) sc[y >> 4][y & 15] = it ? sc[y >> 4][y & 15] * scale2 - m : sc[y >> 4][y & 15];
+                    if (it) by = 1.f, off = 0.f;
                 }
                 typedef short s4 __attribute__((ext_vector_type(4)));
                 const char *vrow = vb + vr * RB + vb8;
@@ -224,8 +232,8 @@ __global__ __launch_bounds__(64 * RW * KG, DC > 128 || (DC > 64 && RW == 2) ? 1 
                 };
                 // two of a group's eight probabilities, rounded
                 auto p_pair = [&](int u, int y) {
-                    const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[u >> 1][(u & 1) * 8 + 2 * y], scale2, -m));
-                    const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[u >> 1][(u & 1) * 8 + 2 * y + 1], scale2, -m));
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[u >> 1][(u & 1) * 8 + 2 * y], by, -off));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[u >> 1][(u & 1) * 8 + 2 * y + 1], by, -off));
                     return pack2<T>(p0, p1);
                 };
                 unsigned pb[2][4];

@@ -99,6 +99,7 @@ template <int DC, bool FULL, int RW, int KG> __global__ __launch_bounds__(64 * R
 #pragma unroll
             for (int y = 0; y < 16; ++y) o[x][y] = 0.f;
         float m = kNoMax, l = 0.f;
+        bool far = false;
 
         const int64_t from = first.begin + (int64_t)split * g.split_keys, to = split + 1 < g.splits ? from + g.split_keys : final.end;
         const int lo = (int)min(from, (int64_t)final.end), hi = (int)min(to, (int64_t)final.end);
@@ -190,6 +191,14 @@ template <int DC, bool FULL, int RW, int KG> __global__ __launch_bounds__(64 * R
                     m = to, l *= fade;
 #pragma unroll
                     for (int x = 0; x < ND; ++x) o[x] *= fade;
+                    far = __any(is_far(to));
+                }
+                float by = scale2, off = m;
+                if (far) {
+                    const bool it = is_far(m);
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) sc[y] = it ? sc[y] * scale2 - m : sc[y];
+                    if (it) by = 1.f, off = 0.f;
                 }
                 const char *vrow = vb + vr * RB + vb8;
                 const int vswz = v_swz(vr);
@@ -211,7 +220,7 @@ template <int DC, bool FULL, int RW, int KG> __global__ __launch_bounds__(64 * R
                     float p[8];
 #pragma unroll
                     for (int y = 0; y < 8; ++y) {
-                        p[y] = __builtin_amdgcn_exp2f(fmaf(sc[8 * u + y], scale2, -m));
+                        p[y] = __builtin_amdgcn_exp2f(fmaf(sc[8 * u + y], by, -off));
                         l += p[y];
                     }
                     split3(p, pb[u], unused);
