@@ -1,4 +1,5 @@
-"""Attention over a paged cache where scores are far from zero: against closed forms.
+"""Attention over a paged cache where scores are far from zero, or many keys weigh little: against closed forms and
+oracle/decode.py.
 
 u = half a step of the type, f = 2^-24, as in test_decode_gpu.py."""
 import math
@@ -74,3 +75,30 @@ def test_scores_at_the_ends_of_the_range(gpu, dtype, route):
     for a, top, low, scale in ((-2.0 ** 63, big, less, 1.0), (-2.0 ** 63, big, big * 1.5, 1.25), (2.0 ** 63, less, big, 1.0), (2.0 ** 62, big, less, -1.5)):
         c = _far(gpu, dtype, route, a, top, low)
         _is_mean_of_the_top(c, ops.paged_attention(c.q.to(gpu), c.cache, c.batch, scale=scale), dtype, "%g %g %g" % (a, top, scale))
+
+
+@pytest.mark.parametrize("where", ["first", "last"])
+@pytest.mark.parametrize("new,n,kv,heads,dim", [(1, 4096, 1, 8, 64), (1, 9000, 2, 2, 128), (12, 4096, 1, 4, 192), (120, 5000, 1, 2, 64), (33, 4100, 8, 32, 128)])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_many_light_keys_keep_their_weight(gpu, dtype, new, n, kv, heads, dim, where):
+    """One key that outweighs each of the others by e^17.69 = 2^25.5, which only the others' values tell apart from nothing.
+
+    A light key's p rounds to its type: u of itself, or half of the last place of a subnormal, 2^-25 where the heaviest key's is 2^11 at
+    least (fp16): 2^-36 of the heaviest a key."""
+    c = Case(gpu, dtype, [new], [n], kv, heads, dim, 16, seed=5)
+    c.q.zero_()
+    c.q[..., 1] = 8.0
+    heavy = 0 if where == "first" else n - new
+    page, row = _at(c)
+    k, v = torch.zeros(n, kv, dim), torch.rand(n, kv, dim, generator=_g(2)) + 0.5
+    k[..., 1] = -17.6875
+    k[heavy], v[heavy] = 0, 0
+    c.cache.k[page, :, row], c.cache.v[page, :, row] = k.to(dtype).to(gpu), v.to(dtype).to(gpu)
+    got = ops.paged_attention(c.q.to(gpu), c.cache, c.batch, scale=0.125)
+    want, mag, reach = c.want(0.125)
+    delta = (6 * math.sqrt(dim) + 4) * F * reach
+    rel = 2 * delta + 6 * math.sqrt(n) * F + (u(dtype) if dtype != torch.float32 else 0.0) + 8 * F
+    lost = n * 2.0 ** -36 * 1.5 if dtype == torch.float16 else 0.0
+    last = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2                       # half of the last place of a subnormal result
+    assert float(want.abs().min()) > 5e-5
+    _within(got, want, u(dtype) * want.abs() + rel * mag + lost + last, where)

@@ -12,7 +12,7 @@
 // and regroups the halves with one v_perm per pair, so nothing passes through LDS.  fp32 uses the 4-deep fp32 product: no regrouping,
 // 16 keys a tile.
 //
-// The running maximum moves only when a score exceeds it by more than 2^8 (p <= 256 then, within every type's range): the cross-lane
+// The running maximum moves only when a score exceeds it by a good deal (lazy; p stays within every type's range): the cross-lane
 // maximum and the scaling of O are skipped in almost every tile.
 //
 // Where a tile's rows lie (page lookup, one key a lane, keys in lanes 0-31 and values in lanes 32-63) is fetched a tile ahead; a
@@ -37,7 +37,11 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr float kNoMax = -3.402823466e38f;      // a running maximum before the first key: no score lies below it, no difference of two is NaN
 constexpr float kFar = 4194304.f;               // 2^22
-constexpr float kLazy = 8.f;         // how far (log2) a score may exceed the running maximum before it moves
+// How far (log2) a row's largest p lies above 1 when the running maximum moves, and how much further it may rise before it moves again.
+// fp16 holds no step below 2^-24: with a largest p of 2^11 to 2^15 a key loses at most 2^-36 of the heaviest one's weight (from 1 to 2^8,
+// thousands of keys of 2^-25 each weighed nothing).  bf16 and fp32 have the range.
+template <class T> constexpr float lift() { return __is_same(T, _Float16) ? 11.f : 0.f; }
+template <class T> constexpr float lazy() { return __is_same(T, _Float16) ? 4.f : 8.f; }
 
 struct AttArgs {
     ttsamd_paged_attention_args a;
@@ -329,10 +333,10 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
 #pragma unroll
                 for (int e = 1; e < VK; ++e) top = fmaxf(top, sc[u][e >> 2][e & 3]);
                 top *= scale2;
-                if (__any(top > m[u] + kLazy)) {
+                if (__any(top > m[u] + (lift<T>() + lazy<T>()))) {
                     top = fmaxf(top, __shfl_xor(top, 16));
                     top = fmaxf(top, __shfl_xor(top, 32));
-                    const float to = fmaxf(m[u], top), fade = __builtin_amdgcn_exp2f(m[u] - to);
+                    const float to = fmaxf(m[u], top - lift<T>()), fade = __builtin_amdgcn_exp2f(m[u] - to);
                     m[u] = to, l[u] *= fade;
 #pragma unroll
                     for (int x = 0; x < NV; ++x) o[u][x] *= fade;
@@ -528,7 +532,7 @@ template <int DP, bool FULL, int R> __global__ __launch_bounds__(512) void atten
                         if (!ALL) sc[u][i] = masked(sc[u][i], bits, i);
                         top = fmaxf(top, sc[u][i] * scale2);
                     }
-                    if (__any(top > m[u] + kLazy)) {
+                    if (__any(top > m[u] + lazy<float>())) {
                         const float to = fmaxf(m[u], top), fade = __builtin_amdgcn_exp2f(m[u] - to);
                         m[u] = to, l[u] *= fade;
 #pragma unroll

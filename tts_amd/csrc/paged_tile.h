@@ -205,9 +205,9 @@ __global__ __launch_bounds__(64 * RW * KG, DC > 128 || (DC > 64 && RW == 2) ? 1 
 #pragma unroll
                 for (int y = 1; y < 32; ++y) top = fmaxf(top, sc[y >> 4][y & 15]);
                 top *= scale2;
-                if (__any(top > m + kLazy)) {
+                if (__any(top > m + (lift<T>() + lazy<T>()))) {
                     top = fmaxf(top, __shfl_xor(top, 32));
-                    const float to = fmaxf(m, top), fade = __builtin_amdgcn_exp2f(m - to);
+                    const float to = fmaxf(m, top - lift<T>()), fade = __builtin_amdgcn_exp2f(m - to);
                     m = to, l *= fade;
 #pragma unroll
                     for (int x = 0; x < ND; ++x) o[x] *= fade;

@@ -185,7 +185,7 @@ template <int DC, bool FULL, int RW, int KG> __global__ __launch_bounds__(64 * R
 #pragma unroll
                 for (int y = 1; y < 16; ++y) top = fmaxf(top, sc[y]);
                 top *= scale2;
-                if (__any(top > m + kLazy)) {
+                if (__any(top > m + lazy<float>())) {
                     top = fmaxf(top, __shfl_xor(top, 32));
                     const float to = fmaxf(m, top), fade = __builtin_amdgcn_exp2f(m - to);
                     m = to, l *= fade;
