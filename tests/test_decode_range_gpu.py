@@ -102,3 +102,18 @@ def test_many_light_keys_keep_their_weight(gpu, dtype, new, n, kv, heads, dim, w
     last = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2                       # half of the last place of a subnormal result
     assert float(want.abs().min()) > 5e-5
     _within(got, want, u(dtype) * want.abs() + rel * mag + lost + last, where)
+
+
+@pytest.mark.parametrize("new,n,kv,heads,dim", [(1, 60, 2, 4, 64), (1, 1500, 1, 8, 128), (1, 700, 2, 6, 192), (9, 200, 1, 3, 80), (20, 300, 1, 4, 64), (16, 90, 2, 8, 128),
+                                                (30, 400, 2, 4, 256), (1, 3000, 1, 2, 96)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_streamed_rows_keep_their_probabilities(gpu, dtype, new, n, kv, heads, dim):
+    """Rows below the staged kernels' 96: a probability is a part of T and the remainder, rounded to T, u^2 of it off (and half of fp16's
+    last step, 2^-36 of the heaviest key); nothing but the result is rounded to the type once."""
+    c = Case(gpu, dtype, [new], [n], kv, heads, dim, 16, seed=dim)
+    want, mag, reach = c.want(dim ** -0.5)
+    delta = (6 * math.sqrt(dim) + 4) * F * reach
+    rel = 2 * delta + 6 * math.sqrt(n) * F + 8 * F + u(dtype) ** 2
+    lost = n * 2.0 ** -36 * float(c.cache.v[c.table[0].long()].nan_to_num(0, 0, 0).abs().max()) if dtype == torch.float16 else 0.0
+    last = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    _within(ops.paged_attention(c.q.to(gpu), c.cache, c.batch), want, u(dtype) * want.abs() * (1 + rel) + rel * mag + lost + last, "two parts")

@@ -5,12 +5,16 @@
 // a running maximum and sum of its own, and are joined in LDS at the end.
 //
 // Layout.  S^T = K Q^T is computed with the keys as the matrix rows, so that in the 16x16 result a lane holds one query row (column
-// lane % 16) and the keys 4 (lane / 16) + i: maximum, exponential and sum stay in the lane.  The same registers, rounded to T, are the
+// lane % 16) and the keys 4 (lane / 16) + i: maximum, exponential and sum stay in the lane.  The same registers, in T, are the
 // right operand of O^T = V^T P^T as they lie, because the order of the keys inside a contraction is free: slot (lane / 16, e) of the
 // 32-deep product is key 4 (lane / 16) + e of the first 16 keys for e < 4, of the second for e >= 4.  The left operand V^T wants, per
 // lane, eight keys of one channel; a lane loads eight keys of NV = DP / 16 neighbouring channels (16 bytes and whole lines at DP = 128)
 // and regroups the halves with one v_perm per pair, so nothing passes through LDS.  fp32 uses the 4-deep fp32 product: no regrouping,
 // 16 keys a tile.
+//
+// A probability travels in two parts of T, the nearest one and the remainder, a product each (together 16 bits of bf16, 22 of fp16), and is
+// summed in fp32: rounded to T once it would be off by as much as the result's own rounding.  These kernels wait for memory: 48 fp16 tokens
+// over 1007 keys 32.3 -> 32.8 us, three bf16 ones over 65537 77.6 -> 77.7, eight sequences of 40 rows over 2000 keys 24.7 -> 25.6.
 //
 // The running maximum moves only when a score exceeds it by a good deal (lazy; p stays within every type's range): the cross-lane
 // maximum and the scaling of O are skipped in almost every tile.
@@ -81,6 +85,18 @@ template <class T> __device__ __forceinline__ unsigned pack2(float x, float y)
     typedef float f2 __attribute__((ext_vector_type(2)));
     typedef T t2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f2{x, y}), t2));
+}
+// x and y in two parts of T each: the nearest one and what it leaves, rounded.
+template <class T> __device__ __forceinline__ void split2(float x, float y, unsigned &upper, unsigned &lower)
+{
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    upper = pack2<T>(x, y);
+    if constexpr (__is_same(T, __bf16)) {
+        lower = pack2<T>(x - __uint_as_float(upper << 16), y - __uint_as_float(upper & 0xffff0000u));
+    } else {
+        const t2 h = __builtin_bit_cast(t2, upper);
+        lower = pack2<T>(x - (float)h[0], y - (float)h[1]);
+    }
 }
 // Both halves of w, added to c in fp32: the probabilities as the products take them, so that what their rounding does to numerator and
 // denominator alike falls out.
@@ -364,25 +380,28 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
                         for (int u = 0; u < NQ; ++u)
                             o[u][x] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[e][x]), p[u][e], o[u][x], 0, 0, 0);
             } else if constexpr (KT == 16) {
-                uint2 pb[NQ];
+                uint2 pb[NQ][2];
 #pragma unroll
                 for (int u = 0; u < NQ; ++u) {
-                    pb[u] = uint2{pack2<T>(p[u][0], p[u][1]), pack2<T>(p[u][2], p[u][3])};
-                    l[u] = sum2<T>(pb[u].x, sum2<T>(pb[u].y, l[u]));
+                    split2<T>(p[u][0], p[u][1], pb[u][0].x, pb[u][1].x), split2<T>(p[u][2], p[u][3], pb[u][0].y, pb[u][1].y);
+#pragma unroll
+                    for (int e = 0; e < VK; ++e) l[u] += p[u][e];
                 }
 #pragma unroll
                 for (int x = 0; x < NV; ++x) {
                     const unsigned sel = x & 1 ? 0x07060302u : 0x05040100u;
                     const uint2 vt = {__builtin_amdgcn_perm(v[1][x / 2], v[0][x / 2], sel), __builtin_amdgcn_perm(v[3][x / 2], v[2][x / 2], sel)};
 #pragma unroll
-                    for (int u = 0; u < NQ; ++u) o[u][x] = mfma_16x16x16<T>(vt, pb[u], o[u][x]);
+                    for (int u = 0; u < NQ; ++u) o[u][x] = mfma_16x16x16<T>(vt, pb[u][0], mfma_16x16x16<T>(vt, pb[u][1], o[u][x]));
                 }
             } else {
-                uint4 pb[NQ];
+                uint4 pb[NQ][2];
 #pragma unroll
                 for (int u = 0; u < NQ; ++u) {
-                    pb[u] = uint4{pack2<T>(p[u][0], p[u][1]), pack2<T>(p[u][2], p[u][3]), pack2<T>(p[u][4], p[u][5]), pack2<T>(p[u][6], p[u][7])};
-                    l[u] = sum2<T>(pb[u].x, sum2<T>(pb[u].y, sum2<T>(pb[u].z, sum2<T>(pb[u].w, l[u]))));
+                    split2<T>(p[u][0], p[u][1], pb[u][0].x, pb[u][1].x), split2<T>(p[u][2], p[u][3], pb[u][0].y, pb[u][1].y);
+                    split2<T>(p[u][4], p[u][5], pb[u][0].z, pb[u][1].z), split2<T>(p[u][6], p[u][7], pb[u][0].w, pb[u][1].w);
+#pragma unroll
+                    for (int e = 0; e < VK; ++e) l[u] += p[u][e];
                 }
 #pragma unroll
                 for (int x = 0; x < NV; ++x) {
@@ -390,7 +409,7 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
                     const uint4 vt = {__builtin_amdgcn_perm(v[1][x / 2], v[0][x / 2], sel), __builtin_amdgcn_perm(v[3][x / 2], v[2][x / 2], sel),
                                       __builtin_amdgcn_perm(v[5][x / 2], v[4][x / 2], sel), __builtin_amdgcn_perm(v[7][x / 2], v[6][x / 2], sel)};
 #pragma unroll
-                    for (int u = 0; u < NQ; ++u) o[u][x] = mfma_16x16x32<T>(vt, pb[u], o[u][x]);
+                    for (int u = 0; u < NQ; ++u) o[u][x] = mfma_16x16x32<T>(vt, pb[u][0], mfma_16x16x32<T>(vt, pb[u][1], o[u][x]));
                 }
             }
         }

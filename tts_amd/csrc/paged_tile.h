@@ -11,6 +11,11 @@
 // so that the reads of 8 (and 16) neighbouring lanes fall on different banks: keys are read a piece a row down a column, values 32 (64)
 // bytes of four rows.
 //
+// The probabilities are rounded to the type for the second product, numerator and denominator alike: a result is off by up to half a step
+// of the type of sum p |v|, as large as its own rounding (bf16, two chunks of 2048 behind 6143 others: 0.0017 -> 0.0023 of its size in the
+// mean).  A second part, as paged_stream.h takes one, would cost another product for every two: 571 -> 713 us there, 46 -> 55 us for 1000
+// tokens over 2000 keys.
+//
 // Bound: the issue of instructions, 36 cycles a matrix one and 4 any other (the matrix unit is busy for some 40 % of the time, no bank
 // conflicts): two chunks of 2048 bf16 tokens behind 6143 others, 32 heads over 8 of 128: 402 GFLOP in 450 us, 895 TFLOP/s, where 392 us are
 // the sum of its instructions.  Reads AHEAD by 2, 3 or 6 products instead of 4, eight waves a workgroup and raised wave priorities gave
