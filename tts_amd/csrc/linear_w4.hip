@@ -1,10 +1,12 @@
 // Products of a few rows with 4-bit weights: y[m,n] = sum_g s[n,g] sum_{k in g} x[m,k] (level[n,k] - z[n,g]) + bias[n].
 //
-// Mathematics.  A level q becomes a 16-bit float without arithmetic: its four bits put into the top of the mantissa of 16.0 give 16 + q,
-// exact in bf16 and fp16 alike, two levels for one shift and one and-or (the image keeps the levels of a word in the order in which the
-// pairs come out).  The matrix unit sums x (16 + q) over a group in fp32, and x -(16 + z) beside it (a right operand of one value), and
-// the group's scale multiplies what that leaves: no product is rounded before the sum, and what cancels is at most some six times the
-// result's own size.
+// Mathematics.  The matrix unit sums x (q - z) over a group in fp32, and the group's scale multiplies the sum: q - z is a small integer,
+// exact in bf16 and fp16 alike, so no product is rounded, and the sum is no larger on its way than the products are.  (Sums of x q, or of x
+// with an offset level, less z times the sum of x would round at the size of the sum of x: weights at the zero point would weigh.)
+// fp16: the four bits of a level at the end of the mantissa of 1024.0 give 1024 + q, four bits further up in 64.0 64 + q, two levels for one
+// and-or (and a shift for every second pair), less 1024 + z or 64 + z in one packed subtraction.  bf16 has none: a level as the low bits of a
+// byte is q 2^-9 in fp8 (e4m3, the subnormals and the first binade), four bytes of a word a mask, two levels a conversion to fp32, and one
+// fma a level takes 2^9 and z: nineteen instructions a word of eight, against nine.
 // fp32 rows travel as three bf16 parts cut off one after the other (8 + 8 + 8 bits: exact), three products each; up to five rows put their
 // parts beside each other into the sixteen rows of one product (8128 -> 1688, one row: 12.3 -> 10.0 us).
 //
@@ -18,6 +20,8 @@
 // Bound: HBM by its bytes (0.5 + scale / group a weight) once the layer is large (8192 x 8192, group 128, one fp16 row: 34.6 MB in 8.4 us,
 // 4.1 TB/s), the latency of one workgroup for small layers (1024 x 1024: 3.0 us), unpacking and products from some 16 rows on (64 rows of
 // 8192 x 8192: 30 us, 280 TFLOP/s).
+#include <type_traits>
+
 #include "decode_common.h"
 
 namespace ttsamd {
@@ -25,17 +29,9 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// The eight levels of a word as 16 + q: bits 4p and 16 + 4p of the word hold levels 2p and 2p + 1.  `one` is 16.0 twice, in a vector
-// register (and-or takes one scalar operand, the mask).
-template <bool BF> __device__ __forceinline__ uint4 unpack(unsigned w, unsigned one)
-{
-    constexpr int at = BF ? 3 : 6;                                     // where the mantissa of 16 + q holds q
-    constexpr unsigned mask = 0xfu << at | 0xfu << (at + 16);
-    auto field = [&](int bit) { return ((bit < at ? w << (at - bit) : w >> (bit - at)) & mask) | one; };
-    return uint4{field(0), field(4), field(8), field(12)};
-}
 template <bool BF> __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c)
 {
     if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -43,9 +39,33 @@ template <bool BF> __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4
 }
 // The upper halves of x and y.
 __device__ __forceinline__ unsigned uppers(unsigned x, unsigned y) { return __builtin_amdgcn_perm(y, x, 0x07060302u); }
+// The eight levels of a word less the zero point, as eight 16-bit floats: bits 4p and 16 + 4p of the word hold levels 2p and 2p + 1.
+// fp16 takes two offsets, 1024 and 64, twice each, and the zero point on top of them.
+struct Offset {
+    unsigned low, high;
+};
+__device__ __forceinline__ uint4 unpack(unsigned w, Offset at, const f16x2 (&z)[2])
+{
+    const unsigned w8 = w >> 8;
+    auto low = [&](unsigned v) { return __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, (v & 0x000f000fu) | at.low) - z[0]); };
+    auto high = [&](unsigned v) { return __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, (v & 0x00f000f0u) | at.high) - z[1]); };
+    return uint4{low(w), high(w), low(w8), high(w8)};
+}
+__device__ __forceinline__ uint4 unpack(unsigned w, Offset, const float (&zero)[1])
+{
+    const float z = zero[0];
+    const unsigned even = w & 0x0f0f0f0fu, odd = w >> 4 & 0x0f0f0f0fu;       // bytes: levels 0 4 1 5, and 2 6 3 7
+    auto two = [&](unsigned bytes, auto upper) {
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        const f2 q = __builtin_amdgcn_cvt_pk_f32_fp8(bytes, decltype(upper)::value);
+        return uint2{__float_as_uint(fmaf(q[0], 512.f, -z)), __float_as_uint(fmaf(q[1], 512.f, -z))};
+    };
+    const uint2 a = two(even, std::false_type()), b = two(even, std::true_type()), c = two(odd, std::false_type()), d = two(odd, std::true_type());
+    return uint4{uppers(a.x, b.x), uppers(c.x, d.x), uppers(a.y, b.y), uppers(c.y, d.y)};
+}
 
-// Output n of row m product by product, for a sum that is no number: an infinity takes x (16 + q) and x (16 + z) apart into NaN, and fp32
-// values from 2^123 on can pass fp32's range there, where x times the weight need not.
+// Output n of row m product by product, for a sum that is no number: an infinity leaves NaN in its parts, and fp32 values from 2^123 on can
+// pass fp32's range before the scale, where x times the weight need not.
 template <class T, int GROUP> __device__ float summed(const ttsamd_linear_w4_args &a, int m, int n)
 {
     const T *x = (const T *)a.x + (int64_t)m * a.x_stride;
@@ -81,8 +101,11 @@ template <class T, int NT, int GROUP, int MAXW, bool FEW> __global__ __launch_bo
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int chunks = (a.k + 127) / 128, m0 = blockIdx.y * 16, rows = min(a.m - m0, 16), products = BESIDE ? 3 * rows : rows;
     const int c16 = lane & 15, g4 = lane >> 4, row = 4 * (c16 & 3) + (c16 >> 2);
-    unsigned one = BF ? 0x41804180u : 0x4c004c00u;
-    asm("" : "+v"(one));
+    struct Zero {
+        std::conditional_t<BF, float, f16x2> v[BF ? 1 : 2];
+    };
+    Offset offset = {0x64006400u, 0x54005400u};
+    if constexpr (!BF) asm("" : "+v"(offset.low), "+v"(offset.high));      // in vector registers: and-or takes one scalar operand, the mask
     const uint4 *levels[NT];
     int64_t sg[NT];
 #pragma unroll
@@ -127,7 +150,8 @@ template <class T, int NT, int GROUP, int MAXW, bool FEW> __global__ __launch_bo
             for (int i = 0; i < XI; ++i) fetch_x(f.x[i], c, i);
     };
     auto multiply = [&](Chunk &f, int c) {
-        unsigned word[NT][4], zero[NT][GPC];
+        unsigned word[NT][4];
+        Zero zero[NT][GPC];
         float scale[NT][GPC];
         // x by way of LDS: loaded as it lies (whole lines), read as the products take it
 #pragma unroll
@@ -145,10 +169,9 @@ template <class T, int NT, int GROUP, int MAXW, bool FEW> __global__ __launch_bo
             for (int q = 0; q < GPC; ++q) {
                 const unsigned r = f.scale[u][q];
                 scale[u][q] = wide ? __uint_as_float(r) : brain ? __uint_as_float(r << 16) : (float)__builtin_bit_cast(_Float16, (unsigned short)r);
-                // -(16 + z), exact, in both halves
-                const float z = zeros ? -16.f - (float)f.zero[u][q] : -24.f;
-                if constexpr (BF) zero[u][q] = uppers(__float_as_uint(z), __float_as_uint(z));
-                else zero[u][q] = (unsigned)__builtin_bit_cast(unsigned short, (_Float16)z) * 0x10001u;
+                const float z = zeros ? (float)f.zero[u][q] : 8.f;
+                if constexpr (BF) zero[u][q].v[0] = z;
+                else zero[u][q].v[0] = f16x2{(_Float16)(1024.f + z), (_Float16)(1024.f + z)}, zero[u][q].v[1] = f16x2{(_Float16)(64.f + z), (_Float16)(64.f + z)};
             }
         }
         if (c + 2 * waves < chunks) fetch(f, c + 2 * waves);
@@ -188,15 +211,11 @@ template <class T, int NT, int GROUP, int MAXW, bool FEW> __global__ __launch_bo
 #pragma unroll
             for (int q = 0; q < GPC; ++q) {
                 f32x4 part = {0.f, 0.f, 0.f, 0.f};
-                const uint4 start = {zero[u][q], zero[u][q], zero[u][q], zero[u][q]};
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
-                    const uint4 w = unpack<BF>(word[u][q * PER + j], one);
+                    const uint4 w = unpack(word[u][q * PER + j], offset, zero[u][q].v);
 #pragma unroll
-                    for (int p = 0; p < PARTS; ++p) {
-                        part = mfma<BF>(x[q * PER + j][p], start, part);
-                        part = mfma<BF>(x[q * PER + j][p], w, part);
-                    }
+                    for (int p = 0; p < PARTS; ++p) part = mfma<BF>(x[q * PER + j][p], w, part);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[u][i] = fmaf(part[i], scale[u][q], acc[u][i]);
