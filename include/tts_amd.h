@@ -672,6 +672,8 @@ int ttsamd_linear_interp(float *y, const float *x, int64_t rows, int t_in, int t
  *   time per request, keys and values of all earlier positions kept), which the reference leaves to a third-party library.
  * Token-major tensors [tokens, heads, head_dim]: the last dimension contiguous, tokens and heads at any stride (in elements).
  * All requests of a step travel in one call; sequence b owns the tokens q_starts[b] .. q_starts[b+1]-1.
+ * Rows that a call writes may share no memory with each other or with anything that it reads, but where it says so: an output that
+ * overlaps itself or the rows of another tensor of the call is refused; places of the cache are the caller's to keep apart from k, v and q.
  * ---------------------------------------------------------------------------------------- */
 #define TTSAMD_F32 0
 #define TTSAMD_F16 1
@@ -690,7 +692,7 @@ typedef struct ttsamd_rotary_plan {
 
 typedef struct ttsamd_rotary_args {
     const void *x;
-    void *y;                              /* may be x itself (same strides) */
+    void *y;                              /* may be x itself (same rows, same strides) */
     int64_t x_tstride, x_hstride, y_tstride, y_hstride;
     const void *positions;                /* [tokens] */
     int32_t position_bytes;               /* 4 or 8: int32 or int64; any sign */
@@ -726,7 +728,7 @@ typedef struct ttsamd_kv_append_args {
     const void *k, *v;                    /* [tokens, kv_heads, head_dim] */
     int64_t k_tstride, k_hstride, v_tstride, v_hstride;
     const void *q;                        /* [tokens, q_heads, head_dim], or NULL */
-    void *q_out;                          /* rotated q; may be q itself (same strides) */
+    void *q_out;                          /* rotated q; may be q itself (same rows, same strides) */
     int64_t q_tstride, q_hstride, qo_tstride, qo_hstride;
     const void *positions;
     int32_t position_bytes, tokens, q_heads;
@@ -742,7 +744,7 @@ int ttsamd_kv_append(const ttsamd_kv_append_args *args /* host */, const ttsamd_
  * no two calls that may run at once share one): partial results where a long cache is split over the chip. */
 typedef struct ttsamd_paged_attention_args {
     const void *q;                        /* [tokens, q_heads, head_dim] */
-    void *out;
+    void *out;                            /* may be q itself (same rows, same strides) */
     int64_t q_tstride, q_hstride, o_tstride, o_hstride;
     int32_t tokens, q_heads, causal, window;
     float scale;

@@ -42,6 +42,14 @@ int check_paged_batch(const char *what, const ttsamd_paged_batch *b, int tokens)
     return TTSAMD_OK;
 }
 
+int check_written(const char *what, const char *name, const RowSet &out, const char *from, const RowSet &in, bool in_place)
+{
+    TTSAMD_CHECK_ARG(!rows_meet(out), "%s: rows of %s overlap each other", what, name);
+    TTSAMD_CHECK_ARG((in_place && same_rows(out, in)) || !sets_meet(out, in), "%s: %s overlaps %s%s", what, name, from,
+                     in_place ? " (it may be the same rows, in the same order)" : "");
+    return TTSAMD_OK;
+}
+
 namespace {
 
 // One tensor that moves: source rows, destination rows, and whether they turn.
@@ -251,6 +259,9 @@ extern "C" int ttsamd_rotary(const ttsamd_rotary_args *r, const ttsamd_rotary_pl
         set_error("rotary: %d heads of %d channels (up to 2^20 channels a token)", r->heads, r->head_dim);
         return TTSAMD_ERR_UNSUPPORTED;
     }
+    const RowSet x = rows_of(r->x, r->x_tstride, r->x_hstride, r->tokens, r->heads, r->head_dim, r->dtype);
+    const RowSet y = rows_of(r->y, r->y_tstride, r->y_hstride, r->tokens, r->heads, r->head_dim, r->dtype);
+    if (int rc = check_written("rotary", "y", y, "x", x, true)) return rc;
     MoveArgs a = {};
     a.s[0] = {r->x, r->y, r->x_tstride, r->x_hstride, r->y_tstride, r->y_hstride, 0, r->heads, 1, 0, 0};
     a.plan = *plan;
@@ -275,6 +286,13 @@ extern "C" int ttsamd_kv_append(const ttsamd_kv_append_args *r, const ttsamd_pag
     if ((int64_t)(2 * cache->kv_heads + (r->q ? r->q_heads : 0)) * cache->head_dim > (1 << 20)) {
         set_error("kv_append: more than 2^20 channels a token");
         return TTSAMD_ERR_UNSUPPORTED;
+    }
+    if (r->q) {
+        auto rows = [&](const void *at, int64_t t, int64_t h, int heads) { return rows_of(at, t, h, r->tokens, heads, cache->head_dim, cache->dtype); };
+        const RowSet out = rows(r->q_out, r->qo_tstride, r->qo_hstride, r->q_heads);
+        if (int rc = check_written("kv_append", "q_out", out, "q", rows(r->q, r->q_tstride, r->q_hstride, r->q_heads), true)) return rc;
+        if (int rc = check_written("kv_append", "q_out", out, "k", rows(r->k, r->k_tstride, r->k_hstride, cache->kv_heads), false)) return rc;
+        if (int rc = check_written("kv_append", "q_out", out, "v", rows(r->v, r->v_tstride, r->v_hstride, cache->kv_heads), false)) return rc;
     }
     MoveArgs a = {};
     const int turns = plan && plan->rotary_dim > 0;

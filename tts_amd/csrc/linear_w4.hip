@@ -309,6 +309,9 @@ extern "C" int ttsamd_linear_w4(const ttsamd_linear_w4_args *a, void *stream)
         set_error("linear_w4: %d rows, %d by %d weights (up to 2^20 - 16 rows, 2^30 a side)", a->m, a->n, a->k);
         return TTSAMD_ERR_UNSUPPORTED;
     }
+    if (int rc = check_written("linear_w4", "y", rows_of(a->y, a->y_stride, 0, a->m, 1, a->n, a->dtype), "x",
+                               rows_of(a->x, a->x_stride, 0, a->m, 1, a->k, a->dtype), false))
+        return rc;
     hipStream_t st = as_stream(stream);
     TTSAMD_HIP(a->dtype == TTSAMD_F32 ? start<float>(*a, st) : a->dtype == TTSAMD_F16 ? start<_Float16>(*a, st) : start<__bf16>(*a, st));
     TTSAMD_LAUNCH_CHECK();

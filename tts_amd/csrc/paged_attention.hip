@@ -127,6 +127,9 @@ extern "C" int ttsamd_paged_attention(const ttsamd_paged_attention_args *a, cons
     TTSAMD_CHECK_ARG((((uintptr_t)a->q | (uintptr_t)a->out) & 15) == 0 && a->q_tstride % per == 0 && a->q_hstride % per == 0 &&
                          a->o_tstride % per == 0 && a->o_hstride % per == 0,
                      "paged_attention: q and out start and stride at multiples of 16 bytes");
+    const RowSet q = rows_of(a->q, a->q_tstride, a->q_hstride, a->tokens, a->q_heads, cache->head_dim, cache->dtype);
+    const RowSet out = rows_of(a->out, a->o_tstride, a->o_hstride, a->tokens, a->q_heads, cache->head_dim, cache->dtype);
+    if (int rc = check_written("paged_attention", "out", out, "q", q, true)) return rc;
     const PagedLaunch p = plan_of(*a, *cache, *batch);
     TTSAMD_CHECK_ARG(p.splits == 1 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= p.part_bytes + p.stat_bytes),
                      "paged_attention: a workspace of %zu bytes at a multiple of 16 is wanted", p.part_bytes + p.stat_bytes);

@@ -781,6 +781,7 @@ def sample_gaussian(stats, noise, mask):
 # products with 4-bit weights.  Token-major [tokens, heads, head_dim] tensors in float32, float16 or bfloat16.  Work is queued on
 # the tensors' device, on its current stream.  All of it can be captured into a graph: nothing waits for the device, and sizes
 # that vary from step to step (lengths, starts, the block table) are read there.  Nothing is recorded for autograd.
+# An `out` that overlaps itself (an expanded one) or an input is refused, except where it may be the input itself.
 # ---------------------------------------------------------------------------------------------------------------------
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # TTSAMD_F32 / F16 / BF16
 
@@ -1101,7 +1102,7 @@ def paged_attention(q, cache, batch, scale=None, causal=True, window=0, out=None
     """Attention of q [tokens, q_heads, head_dim] over the cache (`ttsamd_paged_attention`): every new token over the keys of its sequence
     up to itself (causal) and no further back than `window` tokens, itself among them (0: all).  q_heads: a multiple of the cache's heads,
     head h reads key head h // (q_heads // kv_heads).  scale: default head_dim ** -0.5.  A token that sees no key gets zeros; rows of
-    `out` behind the last sequence are left as they were."""
+    `out` (may be q) behind the last sequence are left as they were."""
     dtype, device, dim = cache.dtype, cache.device, cache.head_dim
     shape = q.shape
     if len(shape) != 3 or shape[1] == 0 or shape[1] % cache.kv_heads:
