@@ -37,3 +37,10 @@ def test_nbytes_is_the_images_size():
     levels, groups = tiles * chunks * 256 * 4, tiles * 16 * 4
     assert ops.PackedW4(q, s).nbytes() == levels + 4 * groups
     assert ops.PackedW4(q, s, z, b).nbytes() == levels + 5 * groups + 4 * 40
+
+
+def test_levels_of_other_ranks_are_refused():
+    q, s, z, b = _parts()
+    for bad in (q[0], q[..., None], q[None], torch.zeros((), dtype=torch.uint8)):
+        with pytest.raises(_lib.TtsAmdError, match="qweight"):
+            ops.PackedW4(bad, s)

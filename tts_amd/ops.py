@@ -1140,6 +1140,7 @@ class PackedW4:
     written into them later does not reach the layer."""
 
     def __init__(self, qweight, scales, zeros=None, bias=None):
+        _need(qweight.dim() == 2, "qweight is %s: uint8 [n, k / 2] is wanted" % (list(qweight.shape),))
         n, k = qweight.shape[0], 2 * qweight.shape[1]
         _need(qweight.dtype == torch.uint8 and scales.dtype in _DTYPES and scales.dim() == 2 and scales.shape[0] == n and scales.shape[1] > 0,
               "qweight uint8 [n, k / 2] and scales [n, k / group] in float32, float16 or bfloat16 are wanted")
