@@ -18,9 +18,9 @@ OBJ = os.path.join(HERE, "build" + ("_" + TAG if TAG else ""))
 LIB = os.path.join(HERE, "libtts_amd%s.so" % ("_" + TAG if TAG else ""))
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32.  hipcc forms them from ordinary float code, and some of their forms have given wrong
-# values on this stack now and then; the scalar forms give the same bits and cost nothing (headline step 48.7 against 49.1-49.2 ms
-# on one machine, dominant conv 389 against 380 TFLOP/s).  The host pass does not know the feature and says so: harmless.
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32, which hipcc forms from ordinary float code.  A precaution that costs nothing: some of their
+# forms are not trusted on this stack (no wrong value of this library is known), and the scalar ones give the same bits (headline step 48.7
+# against 49.1-49.2 ms on one machine, dominant conv 389 against 380 TFLOP/s).  The host pass does not know the feature and says so: harmless.
 FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-Wno-unused-result", "-Wno-pass-failed"] + os.environ.get("TTSAMD_EXTRA_FLAGS", "").split()
@@ -35,6 +35,12 @@ def _newer(target, deps):
 
 def build_lib(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
+    # objects are taken over only from a finished build with the same compiler and flags
+    made_with, record = " ".join([HIPCC] + FLAGS), os.path.join(OBJ, "made_with.txt")
+    if not os.path.exists(record) or open(record).read() != made_with:
+        force = True
+    if force and os.path.exists(record):
+        os.remove(record)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")) + glob.glob(os.path.join(CSRC, "*.cpp")))
     hdrs = glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.inc")) + glob.glob(os.path.join(HERE, "..", "include", "*.h"))
     objs, jobs = [], []
@@ -64,6 +70,8 @@ def build_lib(force: bool = False, verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n%s\n%s" % (r.stdout, r.stderr))
+    with open(record, "w") as f:
+        f.write(made_with)
     return LIB
 
 
