@@ -89,3 +89,21 @@ def test_fp32_rows_whose_large_parts_cancel(gpu):
         _within(got, want, 6 * math.sqrt(3 * k) * F * (32 * 2 * 8.0 + want.abs()), "cancelling")
         rms = float(((got.cpu().double() - want) / mag).pow(2).mean().sqrt())
         assert rms <= 2 * F and float(want.abs().mean()) < 0.05, rms                       # a lost second part is 2^-9 of |x|, a third 2^-17
+
+
+@pytest.mark.parametrize("m,n,k,group,zeros", [(300, 200, 512, 64, True), (1000, 70, 256, 128, False), (437, 1024, 1024, 64, True), (64, 8192, 1024, 128, False),
+                                               (33, 4100, 2080, 32, True), (2, 16400, 256, 64, True), (4, 16400, 384, 128, False)])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_many_rows_and_wide_layers(gpu, dtype, m, n, k, group, zeros):
+    """Prompts and batches: products are exact, so that a sum is off by its own roundings (at most three parts and 32 terms a product, the
+    group's scale and the join: six sigma of as many as there are terms) and by the last one."""
+    g = _g(m + n)
+    x = torch.randn(m, k, generator=g).to(dtype)
+    q = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8)
+    s = ((torch.rand(n, k // group, generator=g) + 0.5) / math.sqrt(k)).to(dtype)
+    z = torch.randint(0, 16, (n, k // group), generator=g, dtype=torch.uint8) if zeros else None
+    bias = torch.randn(n, generator=g).to(dtype)
+    got = ops.linear_w4(ops.PackedW4(q.to(gpu), s.to(gpu), None if z is None else z.to(gpu), bias.to(gpu)), x.to(gpu))
+    want, mag = O.linear_w4(x, q, s, z, bias)
+    tol = u(dtype) * want.abs() * (1 + 2 * F) + 6 * math.sqrt(3 * k) * F * mag + 2 * F * (want.abs() + bias.double().abs()) + torch.finfo(dtype).tiny
+    _within(got, want, tol, "rows")

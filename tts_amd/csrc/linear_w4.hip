@@ -277,13 +277,14 @@ template <class T, int NT> hipError_t start(const ttsamd_linear_w4_args &a, hipS
 template <class T> hipError_t start(const ttsamd_linear_w4_args &a, hipStream_t st)
 {
     // Every workgroup reads its rows of x whole: several output tiles a wave read (and, fp32, split) them once, as long as the chip stays
-    // full and the registers hold (fp16, group 128: 8192 x 8192 with 16 rows 11.8 / 10.7 / 15.3 us at 1 / 2 / 4 tiles, with 64 rows 38.7 /
-    // 35.5 / 30.2 us; 4096 -> 2048, 32 rows: 5.1 / 6.1 / 8.5 us; bf16, group 32: 1024 -> 8192, 64 rows 15.9 / 13.2 / 16.2 us; fp32, 8192 x
-    // 8192 with one row 14.9 / 12.1 us).
+    // full and the registers hold.  us at 1 / 2 / 4 tiles, k = 4096, groups of 64: bf16, 16 rows to 4096 outputs (256 tiles) 6.0 / 8.0 /
+    // 12.3, to 8192 8.8 / 8.4 / 12.7, 64 rows to 8192 24.7 / 27.4 / 23.8; fp16, 32 rows to 8192 (1024 tiles) 13.4 / 13.6 / 11.5, to 16384
+    // 24.1 / 25.2 / 22.8; fp32, one row to 4096 6.8 / 8.7, to 8192 10.4 / 9.5, 64 rows to 4096 31.5 / 22.8.  Few rows have nothing to gain
+    // from four: one bf16 row to 16384 11.7 / 11.8 / 13.1, k = 2048 to 32768 14.1 / 12.3 / 15.4.
     const int64_t tiles = (int64_t)((a.n + 15) / 16) * ((a.m + 15) / 16);
     if (tiles < 512) return start<T, 1>(a, st);
     if constexpr (sizeof(T) == 2)
-        if (tiles >= 1024 && a.group >= 64) return a.group == 64 ? start<T, 4, 64>(a, st) : start<T, 4, 128>(a, st);
+        if (tiles >= 1024 && a.m > few_rows<T>() && a.group >= 64) return a.group == 64 ? start<T, 4, 64, false>(a, st) : start<T, 4, 128, false>(a, st);
     return start<T, 2>(a, st);
 }
 
