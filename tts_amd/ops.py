@@ -1016,7 +1016,8 @@ class PagedKV:
         ks, vs = _inner(k.stride()[:3], k.shape), _inner(v.stride()[:3], v.shape)
         _need(all(s % per == 0 for s in ks + vs) and k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0,
               "rows of the cache have to start at multiples of 16 bytes")
-        self.k, self.v, self.dtype, self.device = k, v, k.dtype, k.device
+        # names of their own for the given memory: it stays where the addresses say, whatever becomes of the caller's tensors
+        self.k, self.v, self.dtype, self.device = k.detach(), v.detach(), k.dtype, k.device
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, rows, dim
         self._scale = dim ** -0.5
         self._c = _PagedKV(k.data_ptr(), v.data_ptr(), *ks, *vs, _DTYPES[k.dtype], pages, heads, rows, dim)
@@ -1044,7 +1045,7 @@ class PagedBatch:
         _need(seq_lens.device == block_table.device == q_starts.device, "block_table, seq_lens and q_starts are on one device")
         _need(batch <= 65535, "%d sequences: up to 65535" % batch)
         _need(0 <= int(max_new) < 2 ** 31 and (max_len is None or 0 <= int(max_len) < 2 ** 31), "max_new and max_len: 0 .. 2^31 - 1")
-        self.block_table, self.seq_lens, self.q_starts = block_table, seq_lens, q_starts
+        self.block_table, self.seq_lens, self.q_starts = block_table.detach(), seq_lens.detach(), q_starts.detach()     # as in PagedKV
         self.batch, self.max_new, self.device = batch, int(max_new), seq_lens.device
         self._c = _PagedBatch(block_table.data_ptr(), block_table.stride(0) if batch > 1 else 0, seq_lens.data_ptr(), q_starts.data_ptr(),
                               block_table.shape[1], batch, self.max_new, 0 if max_len is None else int(max_len))
