@@ -668,8 +668,10 @@ int ttsamd_linear_interp(float *y, const float *x, int64_t rows, int t_in, int t
 
 /* ------------------------------------------------------------------------------------------
  * Autoregressive decoding: the operators of a decoder layer's step over a paged key/value cache.
- * serves: the GPT half of XTTS streaming (TTS/tts/models/xtts.py:610-692: one chunk for the prompt, then one audio token at a
- *   time per request, keys and values of all earlier positions kept), which the reference leaves to a third-party library.
+ * serves: a host that makes the latents which the streaming vocoder reads (TTS/tts/models/xtts.py:610-692: one chunk for the prompt,
+ *   then one audio token at a time per request, keys and values of all earlier positions kept; the reference leaves the model to a
+ *   third-party library).  The reference's own model learns its positions and has a key head for every query head: it takes the
+ *   cache, the attention and the 4-bit products; rotary positions and grouped heads are for models that have them.
  * Token-major tensors [tokens, heads, head_dim]: the last dimension contiguous, tokens and heads at any stride (in elements).
  * All requests of a step travel in one call; sequence b owns the tokens q_starts[b] .. q_starts[b+1]-1.
  * Rows that a call writes may share no memory with each other or with anything that it reads, but where it says so: an output that
@@ -739,7 +741,8 @@ int ttsamd_kv_append(const ttsamd_kv_append_args *args /* host */, const ttsamd_
 /* Attention of the new tokens over the cache: out[t,h] = softmax_j(scale * q[t,h] . k_j) v_j over the keys j of t's sequence that
  * hold a key, with j <= p when causal != 0 and j > p - window when window > 0; p = t's position.  Query head h reads key head
  * h / (q_heads / kv_heads).  A row that sees no key is zero.  Rows of `out` behind the last sequence are left as they were.
- * Statistics and sums in fp32; scores up to 2^127 in size.  head_dim a multiple of 8 up to 256; q, out and the cache start and stride at 16 bytes.
+ * Statistics and sums in fp32 (chunks of 16-bit types round each probability to the type for its product); sums q.k and scores up to
+ * 2^127 in size.  head_dim a multiple of 8 up to 256; q, out and the cache start and stride at 16 bytes.
  * `workspace` (device, ttsamd_paged_attention_workspace_bytes, at most 256 MiB; 16-byte aligned; nothing is kept in it between calls, and
  * no two calls that may run at once share one): partial results where a long cache is split over the chip. */
 typedef struct ttsamd_paged_attention_args {

@@ -6,9 +6,10 @@
 // position (fp32 angles are off by 0.06 rad at p = 10^6, and a table of angles would be as many bytes as a small batch itself).  Its
 // top 32 bits give the nearest quarter turn and a remainder in [-1/8, 1/8] turn, where the Taylor sums of degree 9 / 10 are off by
 // less than 2e-9.
-// Bound: HBM (one read, one write of every byte) once a call moves more than a few MB: 8192 tokens of 32 fp32 heads of 128, 268 MB in
-// 60 us (4.5 TB/s; a copy of that size reaches 5.0 to 5.3), 6 ragged bf16 prompts of up to 1500 tokens with 32 + 2 x 8 heads of 128, 205 MB
-// in 50 us (4.1 TB/s).  Launch latency below: 4 us.  A thread owns one chunk of pairs (two 16-byte pieces) and walks several heads with it,
+// Bound: memory (one read, one write of every byte) once a call moves more than a few MB: 8192 tokens of 32 fp32 heads of 128, 268 MB in
+// 65 us where several such sets take turns (4.1 TB/s; a copy of that size reaches 5.0 to 5.3), 51 where one partly stays in the last-level
+// cache; 6 ragged bf16 prompts of up to 1500 tokens with 32 + 2 x 8 heads of 128, 205 MB in 54 us (3.8 TB/s) and 38.  Launch latency
+// below: 4 us.  A thread owns one chunk of pairs (two 16-byte pieces) and walks several heads with it,
 // because the angles are the same in every head of a token and cost about thirty instructions a pair.
 #include "decode_common.h"
 

@@ -8,7 +8,7 @@
 // byte is q 2^-9 in fp8 (e4m3, the subnormals and the first binade), four bytes of a word a mask, two levels a conversion to fp32, and one
 // fma a level takes 2^9 and z: nineteen instructions a word of eight, against nine.
 // fp32 rows travel as three bf16 parts cut off one after the other (8 + 8 + 8 bits: exact), three products each; up to five rows put their
-// parts beside each other into the sixteen rows of one product (8128 -> 1688, one row: 12.3 -> 10.0 us).
+// parts beside each other into the sixteen rows of one product (8128 -> 1688, one row: 12.3 -> 10.0 us; 10.6 with exact levels).
 //
 // Layout.  16x16x32 products with x as the left operand and 16 outputs as the right one: a lane holds the word of 8 levels of output
 // lane % 16, and 16 bytes of the image are the lane's words of four products (128 k): whole lines, read once, straight into registers.
@@ -17,9 +17,10 @@
 // up to four rows land in one accumulator register of every lane.
 // A workgroup owns 16 outputs; its waves take the chunks of 128 k in turn and are joined in LDS.
 //
-// Bound: HBM by its bytes (0.5 + scale / group a weight) once the layer is large (8192 x 8192, group 128, one fp16 row: 34.6 MB in 8.4 us,
-// 4.1 TB/s), the latency of one workgroup for small layers (1024 x 1024: 3.0 us), unpacking and products from some 16 rows on (64 rows of
-// 8192 x 8192: 30 us, 280 TFLOP/s).
+// Bound: memory by its bytes (0.5 + scale / group a weight) once the layer is large (8192 x 8192, group 128, one fp16 row: 34.6 MB in 10.3
+// us where many layers take turns, 3.4 TB/s, 9.0 over and over; bf16 10.8, fp32 14.4: its unpacking, and for fp32 the parts of x, come on
+// top), the latency of one workgroup for small layers (1024 x 1024: 3.2 us), unpacking and products from some 16 rows on, for every sixteen
+// rows anew (64 rows of 8192 x 8192: fp16 29 us, 295 TFLOP/s, bf16 35, fp32 77).
 #include <type_traits>
 
 #include "decode_common.h"

@@ -25,8 +25,9 @@
 // A value that is an infinity or NaN must not reach rows that do not see its key, and 0 * infinity would: where a tile is seen by some
 // rows only and holds such a value, the rows are computed again key by key.
 //
-// Bound: HBM for single tokens.  48 fp16 sequences of up to 1007 keys, 16 heads of 64: 150 MB in 31.5 us (4.8 TB/s); three bf16 ones of up
-// to 65537, 32 heads over 4 of 128: 363 MB in 66 us (5.5 TB/s; a large copy reaches 5.0 to 5.3), and 5 for the join of 21 splits.
+// Bound: memory for single tokens.  48 fp16 sequences of up to 1007 keys, 16 heads of 64: 150 MB in 33.8 us where many caches take turns
+// (4.4 TB/s), 27.6 where one stays in the last-level cache; three bf16 ones of up to 65537, 32 heads over 4 of 128: 363 MB in 66 us (5.5
+// TB/s; a large copy reaches 5.0 to 5.3), and 5 for the join of 21 splits.
 #pragma once
 #include <type_traits>
 
@@ -447,7 +448,7 @@ __global__ __launch_bounds__(MAXW * 64) void attend_stream(AttArgs g)
 }
 
 // One or two fp32 rows: the same stream without the matrix unit, whose fp32 products of 16 rows would leave 14 of them idle at 1152 cycles
-// a tile of 16 keys of 64 channels, against some 330 here (one token over 605 keys of 16 heads of 64: 6.9 us a launch of a graph).  A lane holds
+// a tile of 16 keys of 64 channels, against some 330 here (one token over 605 keys of 16 heads of 64: 7.3 us a launch of a graph).  A lane holds
 // four channels of every 64 of keys 4 (lane / 16) + i: whole rows of 16 lanes add up a score by rotation, so that the lanes of a key know
 // it, and each 16 lanes keep a maximum, sum and output of their own until the end.
 template <int DP, bool FULL, int R> __global__ __launch_bounds__(512) void attend_few(AttArgs g)

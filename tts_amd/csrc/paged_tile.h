@@ -17,8 +17,8 @@
 // tokens over 2000 keys.
 //
 // Bound: the issue of instructions, 36 cycles a matrix one and 4 any other (the matrix unit is busy for some 40 % of the time, no bank
-// conflicts): two chunks of 2048 bf16 tokens behind 6143 others, 32 heads over 8 of 128: 402 GFLOP in 450 us, 895 TFLOP/s, where 392 us are
-// the sum of its instructions.  Reads AHEAD by 2, 3 or 6 products instead of 4, eight waves a workgroup and raised wave priorities gave
+// conflicts): two chunks of 2048 bf16 tokens behind 6143 others, 32 heads over 8 of 128: 402 GFLOP in 440 to 470 us a call, 860 to 910
+// TFLOP/s (526 in the median of a trace: the clock gives way), where 392 us are the sum of its instructions at the full clock.  Reads AHEAD by 2, 3 or 6 products instead of 4, eight waves a workgroup and raised wave priorities gave
 // nothing.
 #pragma once
 #include "paged_launch.h"

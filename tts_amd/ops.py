@@ -1201,7 +1201,7 @@ class PackedW4:
 
 def linear_w4(weights, x, out=None):
     """x [rows, k] times the packed weights [n, k] transposed, plus their bias -> [rows, n] in x's type (float32, float16, bfloat16).
-    Meant for the few rows of a decoding step; any number is computed."""
+    Meant for the few rows of a decoding step; up to 2^20 - 16 are computed, every sixteen of them reading the weights anew."""
     w = weights
     shape, dtype, device = x.shape, x.dtype, w.device
     kind = _DTYPES.get(dtype)
